@@ -160,6 +160,60 @@ int t2r_gated_ffn_w8a8(int act, const int8_t* w1, const float* s_w1, const int8_
 /* First index of the largest value of each row (np.argmax; llm/ref_model.py:277). */
 int t2r_argmax(const float* x, int rows, int n, int32_t* idx, void* stream);
 
+/* ------------------------------------------- the block-scaled KV cache and what a caller asks of logits
+ * No counterpart in the reference, whose cache has one calibrated scale a layer (or channel). Values are fp32, bf16 or
+ * fp16 (dtype below); sums, softmax statistics and scales are fp32. */
+enum { T2R_F32 = 0, T2R_BF16 = 1, T2R_F16 = 2 };
+/* The cache: int8 codes in a pool of n_blocks blocks of `block` tokens (16, 32, 64 or 128) with one fp32 scale for each
+ * block and KV head, and a table of which block holds which tokens of a sequence:
+ *   kc [n_blocks, Hk, block, hd], ks [n_blocks, Hk]: key   = F(code * scale)
+ *   vc [n_blocks, Hk, hd, block], vs [n_blocks, Hk]: value = F(code * scale)   (by channel: the attention reads along tokens)
+ *   table [B, width]: position p of sequence b lies in block table[b, p / block], slot p % block.
+ * hd <= 128 and a multiple of 16; kc and vc start on 16 bytes. A table entry outside [0, n_blocks), and a place past the
+ * table, holds no tokens: appended rows are dropped there, the attention leaves its positions out, reads give zeros.
+ * A block that is appended to belongs to one sequence (full blocks may be shared by tables).
+ * Ragged rows: those of sequence b are starts[b] .. starts[b + 1] - 1 (starts [B + 1], device, not decreasing) and the
+ * last of them stands at position lens[b] - 1 (device); rows outside every sequence are left alone.
+ *
+ * Appends rows k, v [rows, Hk * hd], k_ld / v_ld elements apart (columns of a q | k | v matrix, say). In each block and
+ * head that rows enter: s = F(max |x| / 127) over its new rows, or its present scale where that is larger and the block
+ * holds earlier tokens of the sequence (its slots below the first new row's); a code is x / s, the real quotient, to the
+ * nearest integer with ties to even; where the scale grew, earlier codes c become c s_old / s_new rounded the same way.
+ * NaN counts as 0 and gives code 0, an infinity as the largest float. Slots behind the rows keep what they hold. */
+int t2r_kv_append_blk(const void* k, const void* v, int dtype, int64_t k_ld, int64_t v_ld, int8_t* kc, int8_t* vc, float* ks,
+                      float* vs, int n_blocks, int block, int Hk, int hd, const int32_t* table, int width,
+                      const int32_t* starts, const int32_t* lens, int B, int rows, void* stream);
+/* The values of cached positions as rows k, v [rows, Hk * hd] (the positions of the ragged rows; zeros where there is none). */
+int t2r_kv_read_blk(const int8_t* kc, const int8_t* vc, const float* ks, const float* vs, int n_blocks, int block, int Hk,
+                    int hd, const int32_t* table, int width, const int32_t* starts, const int32_t* lens, int B, int rows,
+                    int dtype, void* k, void* v, void* stream);
+/* Attention over that cache, out = softmax(scale q K^T) V, H / Hk <= 32 query heads a KV head; q [.., H * hd] and out of
+ * the same type, q_ld / out_ld elements from row to row (out may be q). scale > 0. A row that sees no position (an idle
+ * sequence, or one whose table has no blocks there) gives zeros.
+ * _decode: row b is sequence b's newest token and sees positions 0 .. lens[b] - 1; B <= 65535.
+ * _prefill: ragged rows, each sees the positions up to its own. A row below position 0 (lens[b] less than the sequence's
+ * rows) has no place in its sequence and gives NaN.
+ * Workspace (device, 16-byte aligned): t2r_attn_blk_workspace_bytes with rows = 0 for _decode; 0 bytes may be NULL. It is
+ * one call's scratch: calls that may overlap need one each. */
+int64_t t2r_attn_blk_workspace_bytes(int B, int rows, int H, int Hk, int hd, int block, int width, int dtype);
+int t2r_attn_blk_decode(const void* q, int dtype, int64_t q_ld, const int8_t* kc, const int8_t* vc, const float* ks,
+                        const float* vs, int n_blocks, int block, int Hk, int hd, const int32_t* table, int width,
+                        const int32_t* lens, int B, int H, float scale, void* out, int64_t out_ld, void* workspace,
+                        int64_t workspace_bytes, void* stream);
+int t2r_attn_blk_prefill(const void* q, int dtype, int64_t q_ld, const int8_t* kc, const int8_t* vc, const float* ks,
+                         const float* vs, int n_blocks, int block, int Hk, int hd, const int32_t* table, int width,
+                         const int32_t* starts, const int32_t* lens, int B, int rows, int H, float scale, void* out,
+                         int64_t out_ld, void* workspace, int64_t workspace_bytes, void* stream);
+/* Log probabilities of logits rows [rows, V], ld elements apart: logprob[r] = log softmax(x[r])[tokens[r]]
+ * (NaN for a token outside [0, V)), entropy[r] = -sum p ln p, and the `top` (<= 32, <= V) largest values in descending order,
+ * the lower index first on ties and a NaN before everything: top_ids, top_logprob [rows, top]. logprob (with tokens) and
+ * entropy may be NULL. Values of -inf have probability 0; a row of nothing else gives -inf and entropy 0, a row with a
+ * NaN or +inf gives NaN. Workspace (device, 16-byte aligned): t2r_logprobs_workspace_bytes; one call's scratch. */
+int64_t t2r_logprobs_workspace_bytes(int rows, int V, int top);
+int t2r_logprobs(const void* logits, int dtype, int64_t ld, const int32_t* tokens, int rows, int V, int top,
+                 float* logprob, float* entropy, int32_t* top_ids, float* top_logprob, void* workspace,
+                 int64_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------- model level */
 /* A decoder resident on the device. Pointers are device pointers except kv_consts (host).
  * Per-layer tensors are stacked with the layer first. */

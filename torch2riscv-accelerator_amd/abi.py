@@ -15,6 +15,7 @@ T2R_ABI_VERSION = 2
 T2R_OK, T2R_EINVAL, T2R_ESHAPE, T2R_ERANGE, T2R_EHIP, T2R_ENOMEM, T2R_ESTATE = 0, -1, -2, -3, -4, -5, -6
 T2R_ADVANCE_POS = 1
 T2R_ATTN_QSUM = 1
+T2R_F32, T2R_BF16, T2R_F16 = 0, 1, 2
 T2R_STATIC_WORKSPACE_BYTES = 16 * 1024 * 1024
 T2R_STATIC_STATE_BYTES = 512 * 1024
 
@@ -74,6 +75,16 @@ _SIGS = {
     "t2r_gated_ffn_w8a8": (c_int, [c_int, P, P, P, P, P, P, c_int, c_int, P, P, P, P]),
     "t2r_moe_route": (c_int, [P, c_int, c_int, c_int, c_int, P, P, P]),
     "t2r_argmax": (c_int, [P, c_int, c_int, P, P]),
+    "t2r_kv_append_blk": (c_int, [P, P, c_int, c_int64, c_int64, P, P, P, P, c_int, c_int, c_int, c_int, P, c_int, P, P,
+                                  c_int, c_int, P]),
+    "t2r_kv_read_blk": (c_int, [P, P, P, P, c_int, c_int, c_int, c_int, P, c_int, P, P, c_int, c_int, c_int, P, P, P]),
+    "t2r_attn_blk_workspace_bytes": (c_int64, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "t2r_attn_blk_decode": (c_int, [P, c_int, c_int64, P, P, P, P, c_int, c_int, c_int, c_int, P, c_int, P, c_int, c_int,
+                                    c_float, P, c_int64, P, c_int64, P]),
+    "t2r_attn_blk_prefill": (c_int, [P, c_int, c_int64, P, P, P, P, c_int, c_int, c_int, c_int, P, c_int, P, P, c_int, c_int,
+                                     c_int, c_float, P, c_int64, P, c_int64, P]),
+    "t2r_logprobs_workspace_bytes": (c_int64, [c_int, c_int, c_int]),
+    "t2r_logprobs": (c_int, [P, c_int, c_int64, P, c_int, c_int, c_int, P, P, P, P, P, c_int64, P]),
     "t2r_model_workspace_bytes": (c_int64, [ctypes.POINTER(ModelDesc), c_int]),
     "t2r_model_create": (c_int, [ctypes.POINTER(ModelDesc), ctypes.POINTER(c_void_p)]),
     "t2r_model_create_static": (c_int, [ctypes.POINTER(ModelDesc), ctypes.POINTER(c_void_p)]),

@@ -1,0 +1,249 @@
+// The block-scaled KV cache, the attention over it and the token log probabilities: the entry points of include/t2r.h.
+// A unit of its own: its kernels' code lies apart from t2r.hip's.
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <cstring>
+
+#include "../../include/t2r.h"
+#include "t2r_blkattn.h"
+#include "t2r_block.h"
+#include "t2r_logprob.h"
+
+using namespace t2r;
+
+namespace {
+
+inline int launched() { return hipGetLastError() == hipSuccess ? T2R_OK : T2R_EHIP; }
+inline long long cdiv(long long a, long long b) { return (a + b - 1) / b; }
+inline size_t elem_size(int dtype) { return dtype == T2R_F32 ? 4 : 2; }
+inline bool dtype_ok(int dtype) { return dtype == T2R_F32 || dtype == T2R_BF16 || dtype == T2R_F16; }
+inline bool misaligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) != 0; }
+
+// f(an element of the type): one instantiation a type
+template <class F>
+int by_type(int dtype, F f) {
+  switch (dtype) {
+    case T2R_F32: return f(float());
+    case T2R_BF16: return f(bf16_t());
+    default: return f(_Float16());
+  }
+}
+
+// the cache's description, checked; T2R_OK or a code
+int cache_args(const int8_t* kc, const int8_t* vc, const float* ks, const float* vs, int n_blocks, int block, int Hk,
+               int hd, const int32_t* table, int width, BlkCache* c) {
+  if (!kc || !vc || !ks || !vs || !table) return T2R_EINVAL;
+  if (misaligned(kc, 16) || misaligned(vc, 16) || misaligned(ks, 4) || misaligned(vs, 4) || misaligned(table, 4)) return T2R_EINVAL;
+  if (block != 16 && block != 32 && block != 64 && block != 128) return T2R_ESHAPE;
+  if (hd <= 0 || hd > 128 || hd % 16 || Hk <= 0 || Hk > 65535 || n_blocks <= 0 || width <= 0) return T2R_ESHAPE;
+  if ((long long)n_blocks * Hk > INT32_MAX || (long long)width * block > INT32_MAX) return T2R_ESHAPE;
+  c->kc = (int8_t*)kc; c->vc = (int8_t*)vc; c->ks = (float*)ks; c->vs = (float*)vs; c->table = table;
+  c->n_blocks = n_blocks; c->Hk = Hk; c->hd = hd; c->lbs = __builtin_ctz((unsigned)block); c->width = width;
+  return T2R_OK;
+}
+
+// (block, head) tiles that `rows` rows of B sequences enter at most: n rows enter up to 1 + ceil((n - 1) / block) blocks
+long long blocks_entered(long long rows, long long B, int block) {
+  const long long s = B < rows ? B : rows, x = rows - s;
+  return s + (x < x / block + s ? x : x / block + s);
+}
+
+// How the step form is cut: `chunk` keys a workgroup, so that the launch has some thousand workgroups as long as a chunk
+// keeps its four waves one step of 64 keys each. The lengths are on the device: the table's width bounds them, and
+// workgroups past a sequence's end return at once.
+struct Cut {
+  int chunk, nsplit, tiles, cols;       // tiles and their columns: the ragged form
+};
+Cut step_cut(int B, int H, int Hk, int block, int width, int dtype) {
+  const long long cap = (long long)width * block;
+  const int heads = dtype == T2R_F32 ? 8 : 16, sets = (H / Hk + heads - 1) / heads;
+  const long long units = (long long)B * Hk * sets;
+  Cut c{256, 1, 0, 0};
+  while (c.chunk < kBaSeg && units * cdiv(cap, c.chunk) > 2048) c.chunk *= 2;
+  c.nsplit = (int)cdiv(cap, c.chunk);
+  return c;
+}
+Cut rows_cut(int B, int rows, int H, int Hk, int block, int width) {
+  const long long cap = (long long)width * block;
+  const int G = H / Hk;
+  Cut c;
+  c.cols = (long long)rows * G <= 32LL * B ? 32 : 64;
+  const int rt = c.cols / G;
+  // every sequence's last tile may be a part of one
+  const long long tiles = rows / rt + (B < rows ? B : rows);
+  c.tiles = (int)tiles;
+  const long long wgs = tiles * Hk;
+  c.chunk = (int)cap;
+  c.nsplit = 1;
+  if (wgs < 512) {
+    const long long want = cdiv(1024, wgs);
+    long long ch = cdiv(cdiv(cap, want), 128) * 128;
+    if (ch < 256) ch = 256;
+    c.chunk = (int)ch;
+    c.nsplit = (int)cdiv(cap, ch);
+  }
+  return c;
+}
+
+bool attn_shape_ok(int H, int Hk) { return Hk > 0 && H > 0 && H % Hk == 0 && H / Hk <= 32; }
+long long part_bytes(long long parts, int hd) { return parts * 4 * (hd + 2); }
+long long step_ws(const Cut& c, int B, int H, int hd) { return c.nsplit > 1 ? part_bytes((long long)B * H * c.nsplit, hd) : 0; }
+long long rows_ws(const Cut& c, int Hk, int hd) {
+  return c.nsplit > 1 ? part_bytes((long long)c.tiles * Hk * c.cols * c.nsplit, hd) : 0;
+}
+
+Cut lp_cut(int rows, int V) {             // chunk: spans a part takes; nsplit: parts
+  const long long spans = cdiv(V, kLpSpan);
+  // a part takes several spans where the rows alone are some thousand workgroups
+  long long per = 1;
+  while (per < spans && (long long)rows * cdiv(spans, per) > 4096) per *= 2;
+  return Cut{(int)per, (int)cdiv(spans, per), 0, 0};
+}
+
+}  // namespace
+
+extern "C" {
+
+int t2r_kv_append_blk(const void* k, const void* v, int dtype, int64_t k_ld, int64_t v_ld, int8_t* kc, int8_t* vc, float* ks,
+                      float* vs, int n_blocks, int block, int Hk, int hd, const int32_t* table, int width,
+                      const int32_t* starts, const int32_t* lens, int B, int rows, void* stream) {
+  if (!k || !v || !starts || !lens || !dtype_ok(dtype)) return T2R_EINVAL;
+  if (misaligned(k, elem_size(dtype)) || misaligned(v, elem_size(dtype)) || misaligned(starts, 4) || misaligned(lens, 4)) return T2R_EINVAL;
+  BlkCache c;
+  if (int rc = cache_args(kc, vc, ks, vs, n_blocks, block, Hk, hd, table, width, &c)) return rc;
+  if (B <= 0 || rows <= 0 || k_ld < (int64_t)Hk * hd || v_ld < (int64_t)Hk * hd) return T2R_ESHAPE;
+  const BlkRows x{k, v, k_ld, v_ld};
+  const Ragged g{starts, lens, B, rows};
+  const dim3 grid((unsigned)blocks_entered(rows, B, block), Hk, 2);
+  return by_type(dtype, [&](auto e) {
+    launch(k_blk_append<decltype(e)>, grid, dim3(kBlkThreads), 0, (hipStream_t)stream, x, g, c);
+    return launched();
+  });
+}
+
+int t2r_kv_read_blk(const int8_t* kc, const int8_t* vc, const float* ks, const float* vs, int n_blocks, int block, int Hk,
+                    int hd, const int32_t* table, int width, const int32_t* starts, const int32_t* lens, int B, int rows,
+                    int dtype, void* k, void* v, void* stream) {
+  if (!k || !v || !starts || !lens || !dtype_ok(dtype)) return T2R_EINVAL;
+  if (misaligned(k, elem_size(dtype)) || misaligned(v, elem_size(dtype)) || misaligned(starts, 4) || misaligned(lens, 4)) return T2R_EINVAL;
+  BlkCache c;
+  if (int rc = cache_args(kc, vc, ks, vs, n_blocks, block, Hk, hd, table, width, &c)) return rc;
+  if (B <= 0 || rows <= 0) return T2R_ESHAPE;
+  const Ragged g{starts, lens, B, rows};
+  const dim3 grid((unsigned)blocks_entered(rows, B, block), Hk, 2);
+  return by_type(dtype, [&](auto e) {
+    using E = decltype(e);
+    launch(k_blk_read<E>, grid, dim3(kBlkThreads), 0, (hipStream_t)stream, g, c, (E*)k, (E*)v);
+    return launched();
+  });
+}
+
+int64_t t2r_attn_blk_workspace_bytes(int B, int rows, int H, int Hk, int hd, int block, int width, int dtype) {
+  if (B <= 0 || rows < 0 || !attn_shape_ok(H, Hk) || hd <= 0 || block <= 0 || width <= 0 || !dtype_ok(dtype)) return -1;
+  return rows == 0 ? step_ws(step_cut(B, H, Hk, block, width, dtype), B, H, hd) : rows_ws(rows_cut(B, rows, H, Hk, block, width), Hk, hd);
+}
+
+int t2r_attn_blk_decode(const void* q, int dtype, int64_t q_ld, const int8_t* kc, const int8_t* vc, const float* ks,
+                        const float* vs, int n_blocks, int block, int Hk, int hd, const int32_t* table, int width,
+                        const int32_t* lens, int B, int H, float scale, void* out, int64_t out_ld, void* workspace,
+                        int64_t workspace_bytes, void* stream) {
+  if (!q || !out || !lens || !dtype_ok(dtype) || !(scale > 0) || scale > 3.0e38f) return T2R_EINVAL;
+  if (misaligned(q, elem_size(dtype)) || misaligned(out, elem_size(dtype)) || misaligned(lens, 4)) return T2R_EINVAL;
+  BlkAttn p;
+  std::memset(&p, 0, sizeof(p));
+  if (int rc = cache_args(kc, vc, ks, vs, n_blocks, block, Hk, hd, table, width, &p.c)) return rc;
+  if (!attn_shape_ok(H, Hk) || B <= 0 || B > 65535 || H > 65535 || q_ld < (int64_t)H * hd || out_ld < (int64_t)H * hd) return T2R_ESHAPE;
+  const Cut cut = step_cut(B, H, Hk, block, width, dtype);
+  if (cut.nsplit > 65535) return T2R_ESHAPE;
+  const long long need = step_ws(cut, B, H, hd);
+  if (need > 0 && (!workspace || workspace_bytes < need || misaligned(workspace, 16))) return T2R_ENOMEM;
+  p.q = q; p.q_ld = q_ld; p.out = out; p.out_ld = out_ld;
+  p.g = Ragged{nullptr, lens, B, B};
+  p.H = H; p.G = H / Hk; p.a = scale * 1.44269504f;
+  p.chunk = cut.chunk; p.nsplit = cut.nsplit;
+  p.ws_o = (float*)workspace;
+  p.ws_ml = p.ws_o + (long long)B * H * cut.nsplit * hd;
+  const hipStream_t st = (hipStream_t)stream;
+  return by_type(dtype, [&](auto e) {
+    using E = decltype(e);
+    const int sets = (p.G + Pieces<E>::kHeads - 1) / Pieces<E>::kHeads;
+    const dim3 grid(Hk * sets, cut.nsplit, B);
+    if (hd <= 64) launch((k_blk_step<E, 64>), grid, dim3(kBaThreads), 0, st, p);
+    else launch((k_blk_step<E, 128>), grid, dim3(kBaThreads), 0, st, p);
+    if (cut.nsplit > 1) launch(k_blk_step_join<E>, dim3(H, B), dim3(kJoinThreads), 0, st, p);
+    return launched();
+  });
+}
+
+int t2r_attn_blk_prefill(const void* q, int dtype, int64_t q_ld, const int8_t* kc, const int8_t* vc, const float* ks,
+                         const float* vs, int n_blocks, int block, int Hk, int hd, const int32_t* table, int width,
+                         const int32_t* starts, const int32_t* lens, int B, int rows, int H, float scale, void* out,
+                         int64_t out_ld, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (!q || !out || !starts || !lens || !dtype_ok(dtype) || !(scale > 0) || scale > 3.0e38f) return T2R_EINVAL;
+  if (misaligned(q, elem_size(dtype)) || misaligned(out, elem_size(dtype)) || misaligned(starts, 4) || misaligned(lens, 4)) return T2R_EINVAL;
+  BlkAttn p;
+  std::memset(&p, 0, sizeof(p));
+  if (int rc = cache_args(kc, vc, ks, vs, n_blocks, block, Hk, hd, table, width, &p.c)) return rc;
+  if (!attn_shape_ok(H, Hk) || B <= 0 || rows <= 0 || q_ld < (int64_t)H * hd || out_ld < (int64_t)H * hd) return T2R_ESHAPE;
+  const Cut cut = rows_cut(B, rows, H, Hk, block, width);
+  if (cut.nsplit > 65535 || (long long)cut.tiles * Hk > INT32_MAX) return T2R_ESHAPE;
+  const long long need = rows_ws(cut, Hk, hd);
+  if (need > 0 && (!workspace || workspace_bytes < need || misaligned(workspace, 16))) return T2R_ENOMEM;
+  p.q = q; p.q_ld = q_ld; p.out = out; p.out_ld = out_ld;
+  p.g = Ragged{starts, lens, B, rows};
+  p.H = H; p.G = H / Hk; p.a = scale * 1.44269504f;
+  p.chunk = cut.chunk; p.nsplit = cut.nsplit;
+  p.ws_o = (float*)workspace;
+  p.ws_ml = p.ws_o + (long long)cut.tiles * Hk * cut.cols * cut.nsplit * hd;
+  const hipStream_t st = (hipStream_t)stream;
+  return by_type(dtype, [&](auto e) {
+    using E = decltype(e);
+    const dim3 grid(cut.tiles * Hk, cut.nsplit), jg(cut.tiles * Hk, cut.cols / 4);
+    if (cut.cols == 32) {
+      if (hd <= 64) launch((k_blk_rows<E, 64, 1>), grid, dim3(kBaThreads), 0, st, p);
+      else launch((k_blk_rows<E, 128, 1>), grid, dim3(kBaThreads), 0, st, p);
+      if (cut.nsplit > 1) launch((k_blk_rows_join<E, 1>), jg, dim3(kBaThreads), 0, st, p);
+    } else {
+      if (hd <= 64) launch((k_blk_rows<E, 64, 2>), grid, dim3(kBaThreads), 0, st, p);
+      else launch((k_blk_rows<E, 128, 2>), grid, dim3(kBaThreads), 0, st, p);
+      if (cut.nsplit > 1) launch((k_blk_rows_join<E, 2>), jg, dim3(kBaThreads), 0, st, p);
+    }
+    return launched();
+  });
+}
+
+int64_t t2r_logprobs_workspace_bytes(int rows, int V, int top) {
+  if (rows <= 0 || V <= 0 || top < 0) return -1;
+  return (long long)rows * lp_cut(rows, V).nsplit * (16 + 8LL * top);
+}
+
+int t2r_logprobs(const void* logits, int dtype, int64_t ld, const int32_t* tokens, int rows, int V, int top,
+                 float* logprob, float* entropy, int32_t* top_ids, float* top_logprob, void* workspace,
+                 int64_t workspace_bytes, void* stream) {
+  if (!logits || !dtype_ok(dtype) || (logprob && !tokens) || (top > 0 && (!top_ids || !top_logprob))) return T2R_EINVAL;
+  if (misaligned(logits, elem_size(dtype)) || misaligned(tokens, 4) || misaligned(logprob, 4) || misaligned(entropy, 4) ||
+      misaligned(top_ids, 4) || misaligned(top_logprob, 4))
+    return T2R_EINVAL;
+  if (rows <= 0 || V <= 0 || ld < V) return T2R_ESHAPE;
+  if (top < 0 || top > kLpMaxTop || top > V) return T2R_ERANGE;
+  const Cut cut = lp_cut(rows, V);
+  if ((long long)rows * cut.nsplit > INT32_MAX) return T2R_ESHAPE;
+  if (!workspace || workspace_bytes < t2r_logprobs_workspace_bytes(rows, V, top) || misaligned(workspace, 16)) return T2R_ENOMEM;
+  LpArgs p;
+  std::memset(&p, 0, sizeof(p));
+  p.x = logits; p.ld = ld; p.tokens = tokens; p.rows = rows; p.V = V; p.top = top;
+  p.spans = cut.chunk; p.parts = cut.nsplit;
+  p.logprob = logprob; p.entropy = entropy; p.top_ids = top_ids; p.top_lp = top_logprob;
+  p.ws_sum = (float*)workspace;
+  p.ws_key = (unsigned long long*)(p.ws_sum + 4LL * rows * cut.nsplit);
+  const hipStream_t st = (hipStream_t)stream;
+  return by_type(dtype, [&](auto e) {
+    using E = decltype(e);
+    launch(k_lp_part<E>, dim3(rows * cut.nsplit), dim3(kLpThreads), 0, st, p);
+    launch(k_lp_join<E>, dim3(rows), dim3(kLpThreads), 0, st, p);
+    return launched();
+  });
+}
+
+}  // extern "C"

@@ -1,7 +1,13 @@
 """Op-level calls on torch device tensors: one C-ABI call (one or two HIP launches) per piece of
 the reference's token list (llm/compile_model.py:147-349), each step for step the DeviceModel
 method it names (llm/ref_model.py:191-255). Inputs must be contiguous tensors on a HIP device
-with the dtypes below; outputs are allocated here (the C-ABI itself never allocates)."""
+with the dtypes below; outputs are allocated here (the C-ABI itself never allocates).
+
+The calls at the end (the block-scaled KV cache, the attention over it, log probabilities) have no counterpart in the
+reference. They take float32, bfloat16 or float16 rows that may lie apart (columns of a larger matrix), run on their
+tensors' own device and use that device's current stream."""
+import math
+
 import torch
 
 from . import abi
@@ -207,3 +213,164 @@ def argmax(x):
     idx = torch.empty(rows, dtype=I32, device=x.device)
     abi.call("t2r_argmax", abi.ptr(x), rows, n, abi.ptr(idx), _s())
     return idx
+
+
+# ------------------------------------------------------------------ the block-scaled KV cache
+_DTYPES = {torch.float32: abi.T2R_F32, torch.bfloat16: abi.T2R_BF16, torch.float16: abi.T2R_F16}
+
+
+def _launch(dev, name, *args):
+    """A C-ABI call on device index dev, its current stream as the last argument."""
+    if dev == torch.cuda.current_device():
+        abi.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            abi.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+
+
+def _same(dev, dtype, what, *ts):
+    for t in ts:
+        if t.dtype != dtype or t.get_device() != dev or not t.is_contiguous():
+            raise ValueError(f"{what}: contiguous {dtype} tensors on the rows' device")
+
+
+def _rows(x, n, what):
+    """(elements from row to row, dtype code, device index) of rows x [rows, n] that may lie apart."""
+    code = _DTYPES.get(x.dtype)
+    if code is None or x.dim() != 2 or x.shape[1] != n or not x.is_cuda:
+        raise ValueError(f"{what}: float32, bfloat16 or float16 rows [rows, {n}] on a HIP device, not {x.dtype} {tuple(x.shape)}")
+    ld, one = x.stride()
+    if one != 1 and n > 1:
+        raise ValueError(f"{what}: the values of a row lie side by side (stride 1, not {one})")
+    return (ld if x.shape[0] > 1 else n), code, x.get_device()
+
+
+def _cache(dev, kc, vc, ks, vs, table):
+    """The cache's arguments of the C-ABI, after a check of its tensors (the layout is block_cache's)."""
+    if kc.dim() != 4 or table.dim() != 2:
+        raise ValueError("cache: kc [blocks, Hk, block, hd], vc [blocks, Hk, hd, block], ks and vs [blocks, Hk], table [B, width]")
+    n, Hk, block, hd = kc.shape
+    if vc.shape != (n, Hk, hd, block) or ks.shape != (n, Hk) or vs.shape != (n, Hk):
+        raise ValueError("cache: kc [blocks, Hk, block, hd], vc [blocks, Hk, hd, block], ks and vs [blocks, Hk]")
+    _same(dev, I8, "cache codes", kc, vc)
+    _same(dev, F32, "cache scales", ks, vs)
+    _same(dev, I32, "block table", table)
+    return (kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), n, block, Hk, hd, table.data_ptr(), table.shape[1])
+
+
+def _ragged(dev, table, starts, lens):
+    B = table.shape[0]
+    _same(dev, I32, "starts and lens", starts, lens)
+    if starts.shape != (B + 1,) or lens.shape != (B,):
+        raise ValueError(f"starts [{B + 1}] and lens [{B}] for a table of {B} sequences")
+    return B
+
+
+def block_cache(n_blocks, Hk, hd, block=64, device="cuda:0"):
+    """An empty block-scaled KV cache of n_blocks blocks of `block` tokens (16, 32, 64 or 128), Hk KV heads of hd (a
+    multiple of 16, at most 128): kc [n_blocks, Hk, block, hd] and vc [n_blocks, Hk, hd, block] int8, ks and vs
+    [n_blocks, Hk] float32. Which block holds which tokens is the caller's table [B, width] int32: position p of sequence
+    b lies in block table[b, p // block], slot p % block; an entry outside the pool (-1) is no block."""
+    z = lambda dt, *shape: torch.zeros(shape, dtype=dt, device=device)
+    return z(I8, n_blocks, Hk, block, hd), z(I8, n_blocks, Hk, hd, block), z(F32, n_blocks, Hk), z(F32, n_blocks, Hk)
+
+
+def kv_append_block(k, v, kc, vc, ks, vs, table, starts, lens):
+    """Rows k, v [rows, Hk * hd] into the cache (t2r_kv_append_blk): those of sequence b are starts[b] .. starts[b + 1] - 1
+    and the last of them gets position lens[b] - 1 (lens counts them). A block's scale for a head is max |x| / 127 over what
+    it holds; it grows with later rows, and the block's earlier codes then move to it. Rows at places that the table has
+    no block for are dropped."""
+    n = kc.shape[1] * kc.shape[3] if kc.dim() == 4 else 0
+    k_ld, code, dev = _rows(k, n, "k")
+    v_ld, vcode, vdev = _rows(v, n, "v")
+    if vcode != code or vdev != dev or v.shape != k.shape:
+        raise ValueError("k and v: rows of one type, shape and device")
+    cache = _cache(dev, kc, vc, ks, vs, table)
+    B = _ragged(dev, table, starts, lens)
+    if k.shape[0] and B:
+        _launch(dev, "t2r_kv_append_blk", k.data_ptr(), v.data_ptr(), code, k_ld, v_ld, *cache, starts.data_ptr(),
+                lens.data_ptr(), B, k.shape[0])
+
+
+def kv_read_block(kc, vc, ks, vs, table, starts, lens, rows, dtype=torch.float32):
+    """The cached values as rows k, v [rows, Hk * hd] (t2r_kv_read_blk): rows starts[b] .. starts[b + 1] - 1 are the last
+    positions of sequence b, up to lens[b] - 1; zeros at places that the table has no block for. rows = starts[-1]; rows
+    past it are not written."""
+    if dtype not in _DTYPES:
+        raise ValueError(f"kv_read_block gives float32, bfloat16 or float16, not {dtype}")
+    if not kc.is_cuda:
+        raise ValueError("op arguments must be contiguous tensors on a HIP device")
+    dev = kc.get_device()
+    cache = _cache(dev, kc, vc, ks, vs, table)
+    B = _ragged(dev, table, starts, lens)
+    k = torch.empty((rows, kc.shape[1] * kc.shape[3]), dtype=dtype, device=kc.device)
+    v = torch.empty_like(k)
+    if rows and B:
+        _launch(dev, "t2r_kv_read_blk", *cache, starts.data_ptr(), lens.data_ptr(), B, int(rows), _DTYPES[dtype],
+                k.data_ptr(), v.data_ptr())
+    return k, v
+
+
+def _attention_block(name, q, cache, starts, lens, H, scale):
+    kc, vc, ks, vs, table = cache
+    hd = kc.shape[3] if kc.dim() == 4 else 0
+    q_ld, code, dev = _rows(q, H * hd, "q")
+    c = _cache(dev, kc, vc, ks, vs, table)
+    rows, B, Hk = q.shape[0], table.shape[0], kc.shape[1]
+    ragged = starts is not None
+    if ragged:
+        _ragged(dev, table, starts, lens)
+    else:
+        _same(dev, I32, "lens", lens)
+        if lens.shape != (B,) or rows != B:
+            raise ValueError(f"one row of q and one length for each of the table's {B} sequences")
+    out = torch.empty((rows, H * hd), dtype=q.dtype, device=q.device)
+    if not rows or not B:
+        return out
+    need = abi.load().t2r_attn_blk_workspace_bytes(B, rows if ragged else 0, H, Hk, hd, kc.shape[2], table.shape[1], code)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
+    scale = 1 / math.sqrt(hd) if scale is None else float(scale)
+    _launch(dev, name, q.data_ptr(), code, q_ld, *c, *((starts.data_ptr(),) if ragged else ()), lens.data_ptr(), B,
+            *((rows,) if ragged else ()), H, scale, out.data_ptr(), H * hd, abi.ptr(ws), max(need, 0))
+    return out
+
+
+def attention_block(q, kc, vc, ks, vs, table, lens, H, scale=None):
+    """Attention of one row a sequence, q [B, H * hd], over positions 0 .. lens[b] - 1 of the block-scaled cache
+    (t2r_attn_blk_decode): softmax(scale q K^T) V with scale 1 / sqrt(hd) unless given; H a multiple of Hk. A row whose
+    sequence is empty gives zeros."""
+    return _attention_block("t2r_attn_blk_decode", q, (kc, vc, ks, vs, table), None, lens, H, scale)
+
+
+def attention_block_prefill(q, kc, vc, ks, vs, table, starts, lens, H, scale=None):
+    """Attention of ragged rows q [rows, H * hd] over the block-scaled cache (t2r_attn_blk_prefill): rows starts[b] ..
+    starts[b + 1] - 1 are the last positions of sequence b, up to lens[b] - 1, already in the cache; each sees the positions
+    up to its own. A row below position 0 (lens[b] less than the sequence's rows) gives NaN; rows past starts[-1] are not
+    written."""
+    return _attention_block("t2r_attn_blk_prefill", q, (kc, vc, ks, vs, table), starts, lens, H, scale)
+
+
+# ------------------------------------------------------------------ log probabilities
+def logprobs(logits, tokens=None, top=0):
+    """Of logits rows [rows, V] (t2r_logprobs): (log softmax at tokens [rows] int32, or None without tokens; the entropy;
+    the ids [rows, top] and the log probabilities of the `top` <= 32 largest, descending, the lower id first on ties), all
+    float32 and int32. A token outside [0, V) gives NaN; logits of -inf have probability 0."""
+    if logits.dim() != 2:
+        raise ValueError("logits: rows [rows, V]")
+    rows, V = logits.shape
+    ld, code, dev = _rows(logits, V, "logits")
+    lp = None
+    if tokens is not None:
+        _same(dev, I32, "tokens", tokens)
+        if tokens.shape != (rows,):
+            raise ValueError(f"one token for each of the {rows} rows")
+        lp = torch.empty(rows, dtype=F32, device=logits.device)
+    ent = torch.empty(rows, dtype=F32, device=logits.device)
+    ids = torch.empty((rows, max(top, 0)), dtype=I32, device=logits.device)
+    val = torch.empty((rows, max(top, 0)), dtype=F32, device=logits.device)
+    if rows:
+        need = abi.load().t2r_logprobs_workspace_bytes(rows, V, top)
+        ws = torch.empty(max(need, 0), dtype=torch.uint8, device=logits.device)
+        _launch(dev, "t2r_logprobs", logits.data_ptr(), code, ld, abi.ptr(tokens), rows, V, top, abi.ptr(lp), ent.data_ptr(),
+                ids.data_ptr(), val.data_ptr(), ws.data_ptr(), max(need, 0))
+    return lp, ent, ids, val
