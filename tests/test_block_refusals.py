@@ -80,9 +80,9 @@ def test_logprobs_refuses():
                      (dict(val=None), abi.T2R_EINVAL), (dict(dtype=-1), abi.T2R_EINVAL), (dict(x=ODD), abi.T2R_EINVAL),
                      (dict(rows=0), abi.T2R_ESHAPE), (dict(V=0), abi.T2R_ESHAPE), (dict(ld=99), abi.T2R_ESHAPE),
                      (dict(top=-1), abi.T2R_ERANGE), (dict(top=33), abi.T2R_ERANGE), (dict(V=2, top=3), abi.T2R_ERANGE),
-                     (dict(ws=None), abi.T2R_ENOMEM), (dict(ws_bytes=10), abi.T2R_ENOMEM)):
+                     (dict(V=20000, ld=20000, ws=None), abi.T2R_ENOMEM), (dict(V=20000, ld=20000, ws_bytes=10), abi.T2R_ENOMEM)):
         assert lib.t2r_logprobs(*{**ok, **kw}.values(), None) == code, kw
-    assert lib.t2r_logprobs_workspace_bytes(0, 5, 0) == -1
+    assert lib.t2r_logprobs_workspace_bytes(0, 5, 0) == -1 and lib.t2r_logprobs_workspace_bytes(1, 5, 0) == 0
 
 
 def test_host_checks():

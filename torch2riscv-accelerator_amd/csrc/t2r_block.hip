@@ -93,11 +93,11 @@ long long rows_ws(const Cut& c, int Hk, int hd) {
   return c.nsplit > 1 ? part_bytes((long long)c.tiles * Hk * c.cols * c.nsplit, hd) : 0;
 }
 
+// Parts of a logits row: as many as give the launch four workgroups a CU, each of whole spans
 Cut lp_cut(int rows, int V) {             // chunk: spans a part takes; nsplit: parts
   const long long spans = cdiv(V, kLpSpan);
-  // a part takes several spans where the rows alone are some thousand workgroups
-  long long per = 1;
-  while (per < spans && (long long)rows * cdiv(spans, per) > 4096) per *= 2;
+  const long long want = cdiv(1024, rows) < kLpMaxParts ? cdiv(1024, rows) : kLpMaxParts;
+  const long long per = cdiv(spans, want < spans ? want : spans);
   return Cut{(int)per, (int)cdiv(spans, per), 0, 0};
 }
 
@@ -215,7 +215,8 @@ int t2r_attn_blk_prefill(const void* q, int dtype, int64_t q_ld, const int8_t* k
 
 int64_t t2r_logprobs_workspace_bytes(int rows, int V, int top) {
   if (rows <= 0 || V <= 0 || top < 0) return -1;
-  return (long long)rows * lp_cut(rows, V).nsplit * (16 + 8LL * top);
+  const Cut cut = lp_cut(rows, V);
+  return cut.nsplit > 1 ? (long long)rows * cut.nsplit * (16 + 8LL * top) : 0;
 }
 
 int t2r_logprobs(const void* logits, int dtype, int64_t ld, const int32_t* tokens, int rows, int V, int top,
@@ -229,7 +230,8 @@ int t2r_logprobs(const void* logits, int dtype, int64_t ld, const int32_t* token
   if (top < 0 || top > kLpMaxTop || top > V) return T2R_ERANGE;
   const Cut cut = lp_cut(rows, V);
   if ((long long)rows * cut.nsplit > INT32_MAX) return T2R_ESHAPE;
-  if (!workspace || workspace_bytes < t2r_logprobs_workspace_bytes(rows, V, top) || misaligned(workspace, 16)) return T2R_ENOMEM;
+  const long long need = t2r_logprobs_workspace_bytes(rows, V, top);
+  if (need > 0 && (!workspace || workspace_bytes < need || misaligned(workspace, 16))) return T2R_ENOMEM;
   LpArgs p;
   std::memset(&p, 0, sizeof(p));
   p.x = logits; p.ld = ld; p.tokens = tokens; p.rows = rows; p.V = V; p.top = top;
@@ -241,7 +243,7 @@ int t2r_logprobs(const void* logits, int dtype, int64_t ld, const int32_t* token
   return by_type(dtype, [&](auto e) {
     using E = decltype(e);
     launch(k_lp_part<E>, dim3(rows * cut.nsplit), dim3(kLpThreads), 0, st, p);
-    launch(k_lp_join<E>, dim3(rows), dim3(kLpThreads), 0, st, p);
+    if (cut.nsplit > 1) launch(k_lp_join<E>, dim3(rows), dim3(kLpThreads), 0, st, p);
     return launched();
   });
 }

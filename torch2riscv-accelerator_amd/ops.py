@@ -6,6 +6,7 @@ with the dtypes below; outputs are allocated here (the C-ABI itself never alloca
 The calls at the end (the block-scaled KV cache, the attention over it, log probabilities) have no counterpart in the
 reference. They take float32, bfloat16 or float16 rows that may lie apart (columns of a larger matrix), run on their
 tensors' own device and use that device's current stream."""
+import functools
 import math
 
 import torch
@@ -221,17 +222,16 @@ _DTYPES = {torch.float32: abi.T2R_F32, torch.bfloat16: abi.T2R_BF16, torch.float
 
 def _launch(dev, name, *args):
     """A C-ABI call on device index dev, its current stream as the last argument."""
-    if dev == torch.cuda.current_device():
+    if dev == torch._C._cuda_getDevice():
         abi.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
             abi.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
 
 
-def _same(dev, dtype, what, *ts):
-    for t in ts:
-        if t.dtype != dtype or t.get_device() != dev or not t.is_contiguous():
-            raise ValueError(f"{what}: contiguous {dtype} tensors on the rows' device")
+def _same(t, dev, dtype, what):
+    if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{what}: a contiguous {dtype} tensor on the rows' device")
 
 
 def _rows(x, n, what):
@@ -245,25 +245,37 @@ def _rows(x, n, what):
     return (ld if x.shape[0] > 1 else n), code, x.get_device()
 
 
+_CACHE = "cache: kc [blocks, Hk, block, hd] and vc [blocks, Hk, hd, block] int8, ks and vs [blocks, Hk] float32, table [B, width] int32"
+
+
 def _cache(dev, kc, vc, ks, vs, table):
-    """The cache's arguments of the C-ABI, after a check of its tensors (the layout is block_cache's)."""
+    """The cache's arguments of the C-ABI and the table's sequences, after a check of its tensors."""
     if kc.dim() != 4 or table.dim() != 2:
-        raise ValueError("cache: kc [blocks, Hk, block, hd], vc [blocks, Hk, hd, block], ks and vs [blocks, Hk], table [B, width]")
+        raise ValueError(_CACHE)
     n, Hk, block, hd = kc.shape
-    if vc.shape != (n, Hk, hd, block) or ks.shape != (n, Hk) or vs.shape != (n, Hk):
-        raise ValueError("cache: kc [blocks, Hk, block, hd], vc [blocks, Hk, hd, block], ks and vs [blocks, Hk]")
-    _same(dev, I8, "cache codes", kc, vc)
-    _same(dev, F32, "cache scales", ks, vs)
-    _same(dev, I32, "block table", table)
-    return (kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), n, block, Hk, hd, table.data_ptr(), table.shape[1])
+    B, width = table.shape
+    if vc.shape != (n, Hk, hd, block) or ks.shape != (n, Hk) or vs.shape != ks.shape:
+        raise ValueError(_CACHE)
+    if kc.dtype is not I8 or vc.dtype is not I8 or ks.dtype is not F32 or vs.dtype is not F32 or table.dtype is not I32:
+        raise ValueError(_CACHE)
+    if not (kc.get_device() == vc.get_device() == ks.get_device() == vs.get_device() == table.get_device() == dev):
+        raise ValueError("cache and table: on the rows' device")
+    if not (kc.is_contiguous() and vc.is_contiguous() and ks.is_contiguous() and vs.is_contiguous() and table.is_contiguous()):
+        raise ValueError("cache and table: contiguous tensors")
+    return (kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), n, block, Hk, hd, table.data_ptr(), width), B
 
 
-def _ragged(dev, table, starts, lens):
-    B = table.shape[0]
-    _same(dev, I32, "starts and lens", starts, lens)
-    if starts.shape != (B + 1,) or lens.shape != (B,):
+@functools.lru_cache(maxsize=1024)
+def _workspace(name, *sizes):
+    """Bytes of workspace that a call of these sizes needs (0 where it refuses them: the call itself then says so)."""
+    return max(getattr(abi.load(), name)(*sizes), 0)
+
+
+def _ragged(dev, B, starts, lens):
+    _same(starts, dev, I32, "starts")
+    _same(lens, dev, I32, "lens")
+    if starts.dim() != 1 or lens.dim() != 1 or starts.numel() != B + 1 or lens.numel() != B:
         raise ValueError(f"starts [{B + 1}] and lens [{B}] for a table of {B} sequences")
-    return B
 
 
 def block_cache(n_blocks, Hk, hd, block=64, device="cuda:0"):
@@ -285,8 +297,8 @@ def kv_append_block(k, v, kc, vc, ks, vs, table, starts, lens):
     v_ld, vcode, vdev = _rows(v, n, "v")
     if vcode != code or vdev != dev or v.shape != k.shape:
         raise ValueError("k and v: rows of one type, shape and device")
-    cache = _cache(dev, kc, vc, ks, vs, table)
-    B = _ragged(dev, table, starts, lens)
+    cache, B = _cache(dev, kc, vc, ks, vs, table)
+    _ragged(dev, B, starts, lens)
     if k.shape[0] and B:
         _launch(dev, "t2r_kv_append_blk", k.data_ptr(), v.data_ptr(), code, k_ld, v_ld, *cache, starts.data_ptr(),
                 lens.data_ptr(), B, k.shape[0])
@@ -301,9 +313,9 @@ def kv_read_block(kc, vc, ks, vs, table, starts, lens, rows, dtype=torch.float32
     if not kc.is_cuda:
         raise ValueError("op arguments must be contiguous tensors on a HIP device")
     dev = kc.get_device()
-    cache = _cache(dev, kc, vc, ks, vs, table)
-    B = _ragged(dev, table, starts, lens)
-    k = torch.empty((rows, kc.shape[1] * kc.shape[3]), dtype=dtype, device=kc.device)
+    cache, B = _cache(dev, kc, vc, ks, vs, table)
+    _ragged(dev, B, starts, lens)
+    k = torch.empty(rows, kc.shape[1] * kc.shape[3], dtype=dtype, device=kc.device)
     v = torch.empty_like(k)
     if rows and B:
         _launch(dev, "t2r_kv_read_blk", *cache, starts.data_ptr(), lens.data_ptr(), B, int(rows), _DTYPES[dtype],
@@ -311,27 +323,28 @@ def kv_read_block(kc, vc, ks, vs, table, starts, lens, rows, dtype=torch.float32
     return k, v
 
 
-def _attention_block(name, q, cache, starts, lens, H, scale):
-    kc, vc, ks, vs, table = cache
-    hd = kc.shape[3] if kc.dim() == 4 else 0
+def _attention_block(q, cache, starts, lens, H, scale):
+    hd = cache[0].shape[3] if cache[0].dim() == 4 else 0
     q_ld, code, dev = _rows(q, H * hd, "q")
-    c = _cache(dev, kc, vc, ks, vs, table)
-    rows, B, Hk = q.shape[0], table.shape[0], kc.shape[1]
-    ragged = starts is not None
-    if ragged:
-        _ragged(dev, table, starts, lens)
+    c, B = _cache(dev, *cache)
+    rows = q.shape[0]
+    if starts is not None:
+        _ragged(dev, B, starts, lens)
     else:
-        _same(dev, I32, "lens", lens)
-        if lens.shape != (B,) or rows != B:
+        _same(lens, dev, I32, "lens")
+        if lens.dim() != 1 or lens.numel() != B or rows != B:
             raise ValueError(f"one row of q and one length for each of the table's {B} sequences")
-    out = torch.empty((rows, H * hd), dtype=q.dtype, device=q.device)
+    where = q.device
+    out = torch.empty(rows, H * hd, dtype=q.dtype, device=where)
     if not rows or not B:
         return out
-    need = abi.load().t2r_attn_blk_workspace_bytes(B, rows if ragged else 0, H, Hk, hd, kc.shape[2], table.shape[1], code)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
-    scale = 1 / math.sqrt(hd) if scale is None else float(scale)
-    _launch(dev, name, q.data_ptr(), code, q_ld, *c, *((starts.data_ptr(),) if ragged else ()), lens.data_ptr(), B,
-            *((rows,) if ragged else ()), H, scale, out.data_ptr(), H * hd, abi.ptr(ws), max(need, 0))
+    need = _workspace("t2r_attn_blk_workspace_bytes", B, 0 if starts is None else rows, H, c[6], hd, c[5], c[9], code)
+    ws = torch.empty(need, dtype=torch.uint8, device=where) if need else None
+    tail = (H, 1 / math.sqrt(hd) if scale is None else float(scale), out.data_ptr(), H * hd, ws.data_ptr() if need else None, need)
+    if starts is None:
+        _launch(dev, "t2r_attn_blk_decode", q.data_ptr(), code, q_ld, *c, lens.data_ptr(), B, *tail)
+    else:
+        _launch(dev, "t2r_attn_blk_prefill", q.data_ptr(), code, q_ld, *c, starts.data_ptr(), lens.data_ptr(), B, rows, *tail)
     return out
 
 
@@ -339,7 +352,7 @@ def attention_block(q, kc, vc, ks, vs, table, lens, H, scale=None):
     """Attention of one row a sequence, q [B, H * hd], over positions 0 .. lens[b] - 1 of the block-scaled cache
     (t2r_attn_blk_decode): softmax(scale q K^T) V with scale 1 / sqrt(hd) unless given; H a multiple of Hk. A row whose
     sequence is empty gives zeros."""
-    return _attention_block("t2r_attn_blk_decode", q, (kc, vc, ks, vs, table), None, lens, H, scale)
+    return _attention_block(q, (kc, vc, ks, vs, table), None, lens, H, scale)
 
 
 def attention_block_prefill(q, kc, vc, ks, vs, table, starts, lens, H, scale=None):
@@ -347,7 +360,7 @@ def attention_block_prefill(q, kc, vc, ks, vs, table, starts, lens, H, scale=Non
     starts[b + 1] - 1 are the last positions of sequence b, up to lens[b] - 1, already in the cache; each sees the positions
     up to its own. A row below position 0 (lens[b] less than the sequence's rows) gives NaN; rows past starts[-1] are not
     written."""
-    return _attention_block("t2r_attn_blk_prefill", q, (kc, vc, ks, vs, table), starts, lens, H, scale)
+    return _attention_block(q, (kc, vc, ks, vs, table), starts, lens, H, scale)
 
 
 # ------------------------------------------------------------------ log probabilities
@@ -359,18 +372,21 @@ def logprobs(logits, tokens=None, top=0):
         raise ValueError("logits: rows [rows, V]")
     rows, V = logits.shape
     ld, code, dev = _rows(logits, V, "logits")
+    where = logits.device
     lp = None
     if tokens is not None:
-        _same(dev, I32, "tokens", tokens)
-        if tokens.shape != (rows,):
+        _same(tokens, dev, I32, "tokens")
+        if tokens.dim() != 1 or tokens.numel() != rows:
             raise ValueError(f"one token for each of the {rows} rows")
-        lp = torch.empty(rows, dtype=F32, device=logits.device)
-    ent = torch.empty(rows, dtype=F32, device=logits.device)
-    ids = torch.empty((rows, max(top, 0)), dtype=I32, device=logits.device)
-    val = torch.empty((rows, max(top, 0)), dtype=F32, device=logits.device)
+        lp = torch.empty(rows, dtype=F32, device=where)
+    if not 0 <= top <= min(V, 32):
+        raise ValueError(f"top {top}: 0 .. {min(V, 32)} of {V} values")
+    ent = torch.empty(rows, dtype=F32, device=where)
+    ids = torch.empty(rows, top, dtype=I32, device=where)
+    val = torch.empty(rows, top, dtype=F32, device=where)
     if rows:
-        need = abi.load().t2r_logprobs_workspace_bytes(rows, V, top)
-        ws = torch.empty(max(need, 0), dtype=torch.uint8, device=logits.device)
+        need = _workspace("t2r_logprobs_workspace_bytes", rows, V, top)
+        ws = torch.empty(need, dtype=torch.uint8, device=where) if need else None
         _launch(dev, "t2r_logprobs", logits.data_ptr(), code, ld, abi.ptr(tokens), rows, V, top, abi.ptr(lp), ent.data_ptr(),
-                ids.data_ptr(), val.data_ptr(), ws.data_ptr(), max(need, 0))
+                ids.data_ptr(), val.data_ptr(), ws.data_ptr() if need else None, need)
     return lp, ent, ids, val
