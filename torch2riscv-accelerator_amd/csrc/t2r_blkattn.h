@@ -17,6 +17,8 @@
 // which key a row stands for is free. Rows are assigned so that a lane ends up with 16 consecutive keys, which are
 // what it needs of P as the second product's operand, against 16 consecutive codes of a V^T row (one 16-byte load).
 #pragma once
+#include <type_traits>
+
 #include "t2r_block.h"
 
 namespace t2r {
@@ -25,6 +27,8 @@ constexpr int kBaThreads = 256, kBaWaves = 4;
 constexpr int kBaSeg = 2048;                 // keys whose table entries and scales lie in LDS at a time
 constexpr float kSlack = 4.0f, kLift = 11.0f;
 constexpr float kNegInf = -__builtin_inff();
+
+T2R_DEV int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 struct BlkAttn {
   const void* q;
@@ -35,6 +39,7 @@ struct BlkAttn {
   Ragged g;                 // step form: row b is sequence b's (starts unused)
   int H, G;                 // heads, heads of a KV head
   float a;                  // softmax scale times log2(e)
+  int order;                // find_piece's, of the tiles
   int chunk, nsplit;        // keys of a workgroup (a multiple of its waves' step, at most kBaSeg when nsplit > 1)
   float* ws_o;              // parts of long rows: [row's column, split, hd] sums, and [.., 2] maxima and weights
   float* ws_ml;
@@ -76,30 +81,65 @@ T2R_DEV float add_ror8(float x) {
   return x + fv((uint32_t)__builtin_amdgcn_update_dpp(0, (int)fb(x), 0x128, 0xF, 0xF, false));
 }
 
-// Fills the segment's LDS tables for keys key0 .. key0 + n - 1 (16 keys an entry; -1: no such block, its keys are left
-// out) and returns the largest V scale among them.
+// What a segment's keys need, 16 keys an entry: the (block, head) tile (-1: no block there, its keys are left out), the K
+// scale, and the V scale as a share of vref: its log2, which goes into the probabilities' exponent, and its inverse, which
+// takes it out of their sum again. (A share below 2^-60 counts as that: its values are nothing beside vref's, the
+// probabilities' sum is right all the same.)
 struct BaSeg {
-  int tb[kBaSeg / 16];
-  float ks[kBaSeg / 16], vs[kBaSeg / 16];
-  float red[kBaWaves];
+  int tb[kBaSeg / 16];                        // (0 where there is none)
+  int seen[kBaSeg / 16];                      // 16, or fewer at the end, or none
+  float ks[kBaSeg / 16], lw[kBaSeg / 16], iw[kBaSeg / 16];
+  float red[8];
+  int holes[8];
 };
-T2R_DEV float seg_load(BaSeg& sg, const BlkCache& c, int b, int head, long long key0, int n) {
+// The tables of the keys key0 .. key0 + n - 1, in whole steps of `step` keys, for the whole workgroup. In parts, so that what
+// a kernel has to load meanwhile is asked for between them: seg_table asks for this thread's table entry; seg_blocks puts the
+// tiles into LDS (a barrier: the codes can be asked for then); seg_scales the scales (a second one), and returns the larger
+// of vref and the V scales among them; *holes: some of the n keys have no block.
+T2R_DEV int seg_table(const BlkCache& c, int b, long long key0, int n) {
   const int tid = threadIdx.x;
-  float m = 0;
-  if (tid * 16 < n) {
-    const int blk = c.block(b, (key0 + tid * 16) >> c.lbs);
-    const long long at = (long long)max(blk, 0) * c.Hk + head;
-    const float ks = c.ks[at], vs = c.vs[at];
-    sg.tb[tid] = blk < 0 ? -1 : (int)at;
-    sg.ks[tid] = ks;
-    sg.vs[tid] = blk < 0 ? 0.0f : vs;
-    m = blk < 0 ? 0.0f : fabsf(vs);
+  return tid * 16 < n ? c.block(b, (key0 + tid * 16) >> c.lbs) : -1;
+}
+T2R_DEV void seg_blocks(BaSeg& sg, const BlkCache& c, int blk, int head, int n, int step) {
+  const int tid = threadIdx.x, entries = (n + step - 1) / step * (step >> 4);
+  if (tid < entries) {
+    sg.tb[tid] = max(blk, 0) * c.Hk + (blk < 0 ? 0 : head);
+    sg.seen[tid] = blk < 0 ? 0 : min(n - tid * 16, 16);
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-  if ((tid & 63) == 0) sg.red[tid >> 6] = m;
   __syncthreads();
-  return fmaxf(fmaxf(sg.red[0], sg.red[1]), fmaxf(sg.red[2], sg.red[3]));
+}
+template <int NW>
+T2R_DEV float seg_scales(BaSeg& sg, const BlkCache& c, int blk, int head, int n, int step, float vref, bool* holes) {
+  const int tid = threadIdx.x, wave = wave_index(), entries = (n + step - 1) / step * (step >> 4);
+  float ks = 0, vs = 0;
+  if (blk >= 0) {
+    const long long at = (long long)blk * c.Hk + head;
+    ks = c.ks[at];
+    vs = c.vs[at];
+  }
+  const float wm = wave_max0(fabsf(vs));
+  const bool hole = __any(tid * 16 < n && blk < 0);
+  if ((tid & 63) == 0) {
+    sg.red[wave] = wm;
+    sg.holes[wave] = hole;
+  }
+  __syncthreads();
+  float m = vref;
+  int any = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    m = fmaxf(m, sg.red[w]);
+    any |= sg.holes[w];
+  }
+  *holes = any != 0;
+  if (tid < entries) {
+    sg.ks[tid] = ks;
+    const float share = m > 0 && blk >= 0 ? fmaxf(vs / m, 0x1p-60f) : 1.0f;
+    sg.lw[tid] = __builtin_amdgcn_logf(share);
+    sg.iw[tid] = 1.0f / share;
+  }
+  __syncthreads();
+  return m;
 }
 
 // ---------------------------------------------------------------- one row a sequence
@@ -114,27 +154,38 @@ __global__ __launch_bounds__(kBaThreads) void k_blk_step(BlkAttn p) {
   __shared__ BaSeg sg;
   __shared__ float s_m[kBaWaves][16], s_l[kBaWaves][16];
   __shared__ float s_o[kBaWaves][16][HD + 4];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, c4 = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_index(), col = lane & 15, c4 = lane >> 4;
   const int sets = (p.G + HW - 1) / HW;
   const int kvh = blockIdx.x / sets, h0 = (blockIdx.x - kvh * sets) * HW, b = blockIdx.z, split = blockIdx.y;
   const int hd = p.c.hd, lbs = p.c.lbs, bmask = (1 << lbs) - 1;
   const int nh = min(HW, p.G - h0);                       // heads of this workgroup
-  const long long len = min((long long)p.g.lens[b], (long long)p.c.width << lbs), k0 = (long long)split * p.chunk;
+  const long long k0 = (long long)split * p.chunk;
+  // everything that needs nothing loaded is asked for at once: the length, the table and q
+  const int blk = seg_table(p.c, b, k0, p.chunk);
+  float x[KU][16];
+  const int hsel = col % HW;
+  {
+    const E* q = (const E*)p.q + (long long)b * p.q_ld + (long long)(kvh * p.G + h0 + min(hsel, nh - 1)) * hd;
+#pragma unroll
+    for (int u = 0; u < KU; ++u) {
+      const int d = u * 64 + c4 * 16;
+      Row16<E>::load(q + (d < hd ? d : 0), x[u]);           // (channels past hd are made zero below)
+    }
+  }
+  const long long len = min((long long)p.g.lens[b], (long long)p.c.width << lbs);
   E* out = (E*)p.out + (long long)b * p.out_ld + (long long)(kvh * p.G + h0) * hd;
   if (k0 >= len) {
     if (split == 0)                                        // nothing to attend to
       for (int i = tid; i < nh * hd; i += kBaThreads) out[i] = narrow<E>(0.0f);
     return;
   }
-  const int n = (int)min((long long)p.chunk, len - k0);
-  const float vref = seg_load(sg, p.c, b, kvh, k0, n);
-  const long long tile = p.c.tile_bytes();
-
+  const int n = (int)min((long long)p.chunk, len - k0), steps = (n + 63) >> 6, tile = p.c.tile_bytes();
+  const int mine = tid * 16 < n ? blk : -1;
   v4i_t kr[4][KU], vr[DT];
   // K rows: row m = 4 c' + r of the t-th 16 stands for key 16 c' + 4 t + r of the 64
   auto load_k = [&](int st) {
-    const int ch = st * 4 + (col >> 2), t = max(sg.tb[ch], 0);
-    const int8_t* base = p.c.kc + t * tile + (long long)(((ch * 16) & bmask) + (col & 3)) * hd;
+    const int ch = st * 4 + (col >> 2);
+    const int8_t* base = p.c.kc + (long long)sg.tb[ch] * tile + (((ch * 16) & bmask) + (col & 3)) * hd;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -144,47 +195,34 @@ __global__ __launch_bounds__(kBaThreads) void k_blk_step(BlkAttn p) {
       }
   };
   auto load_v = [&](int st) {
-    const int ch = st * 4 + c4, t = max(sg.tb[ch], 0);
-    const int8_t* base = p.c.vc + t * tile + ((ch * 16) & bmask);
+    const int ch = st * 4 + c4;
+    const int8_t* base = p.c.vc + (long long)sg.tb[ch] * tile + ((ch * 16) & bmask);
 #pragma unroll
-    for (int i = 0; i < DT; ++i) vr[i] = *(const v4i_t*)(base + ((long long)min(i * 16 + col, hd - 1) << lbs));
+    for (int i = 0; i < DT; ++i) vr[i] = *(const v4i_t*)(base + (min(i * 16 + col, hd - 1) << lbs));
   };
-  // the table holds entries up to the segment's last 16 keys: whole steps of 64 read those past it as "no block"
-  const int steps = (n + 63) >> 6;
-  for (int i = (n + 15) / 16 + tid; i < steps * 4; i += kBaThreads) {
-    sg.tb[i] = -1;
-    sg.ks[i] = 0;
-    sg.vs[i] = 0;
-  }
-  __syncthreads();
+  seg_blocks(sg, p.c, mine, kvh, n, 64);
   int st = wave;
   if (st < steps) {
     load_k(st);
     load_v(st);
   }
-  // q: the row's largest magnitude, then its pieces in the layout of K's rows
+  bool holes;
+  const float vref = seg_scales<kBaWaves>(sg, p.c, mine, kvh, n, 64, 0.0f, &holes);
+  // q's pieces in the layout of K's rows, after the row's largest magnitude
   v8h_t qf[KU][2];
   float sq;
   {
-    const int hsel = col % HW;
-    const E* q = (const E*)p.q + (long long)b * p.q_ld + (long long)(kvh * p.G + h0 + min(hsel, nh - 1)) * hd;
-    float x[KU][16], am = 0;
+    float am = 0;
 #pragma unroll
-    for (int u = 0; u < KU; ++u) {
-      const int d = u * 64 + c4 * 16;
-      Row16<E>::load(q + (d < hd ? d : 0), x[u]);
+    for (int u = 0; u < KU; ++u)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        x[u][i] = d < hd && hsel < nh ? x[u][i] : 0.0f;
-        am = fmaxf(am, fabsf(x[u][i]));
-      }
-    }
+      for (int i = 0; i < 16; ++i) am = fmaxf(am, fabsf(x[u][i]));
     am = fmaxf(am, __shfl_xor(am, 16));
     am = fmaxf(am, __shfl_xor(am, 32));
     const int e = row_exp(am);
-    const float down = pow2i(-e);
 #pragma unroll
-    for (int u = 0; u < KU; ++u)
+    for (int u = 0; u < KU; ++u) {
+      const float down = u * 64 + c4 * 16 < hd ? pow2i(-e) : 0.0f;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float y = held(x[u][i] * down);
@@ -192,13 +230,15 @@ __global__ __launch_bounds__(kBaThreads) void k_blk_step(BlkAttn p) {
         if (NP == 2 && col >= 8) h = (_Float16)(y - (float)h);
         qf[u][i >> 3][i & 7] = h;
       }
+    }
     sq = p.a * pow2i(e);
   }
   float m = kNegInf, l = 0;
   v4f_t o[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i) o[i] = v4f_t{0, 0, 0, 0};
-  for (; st < steps; st += kBaWaves) {
+  // a step of 64 keys; edge: not all of them are seen
+  auto step = [&](auto edge) {
     v4f_t s[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -212,17 +252,16 @@ __global__ __launch_bounds__(kBaThreads) void k_blk_step(BlkAttn p) {
     const bool more = st + kBaWaves < steps;
     if (more) load_k(st + kBaWaves);
     // this lane's 16 keys: 16 c4 + 4 t + r of the 64
-    const int ch = st * 4 + c4, left = sg.tb[ch] < 0 ? 0 : n - ch * 16;
-    const float sk = score_scale(sq, sg.ks[ch]);
-    float wv = 0;
-    if (vref > 0) wv = sg.vs[ch] / vref;
+    const int ch = st * 4 + c4;
+    const float sk = score_scale(sq, sg.ks[ch]), lw = sg.lw[ch], iw = sg.iw[ch];
     if (NP == 2) {
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) s[t][r] = add_ror8(s[t][r]);
     }
-    if (__any(left < 16)) {
+    if constexpr (edge.value) {
+      const int left = sg.seen[ch];
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -243,29 +282,32 @@ __global__ __launch_bounds__(kBaThreads) void k_blk_step(BlkAttn p) {
         for (int i = 0; i < DT; ++i) o[i] *= al;
       }
     }
-    const float sub = (m == kNegInf ? 0.0f : m) - kLift;
+    const float add = lw + kLift - (m == kNegInf ? 0.0f : m);
     v8h_t pf[2];
+    float ls[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], sk, -sub));
-        l += e;
-        const float w = NP == 2 ? held(e * wv) : e * wv;
+        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], sk, add));
+        ls[r] += w;
         _Float16 h = (_Float16)w;
         if (NP == 2) {
-          const _Float16 lo = (_Float16)(w - (float)h);
+          const _Float16 lo = (_Float16)__builtin_fmaf((float)h, -1.0f, w);
           h = col >= 8 ? lo : h;
         }
         pf[t >> 1][(t & 1) * 4 + r] = h;
       }
+    l = __builtin_fmaf((ls[0] + ls[1]) + (ls[2] + ls[3]), iw, l);
 #pragma unroll
     for (int i = 0; i < DT; ++i) {
       o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_h(vr[i][0], vr[i][1]), pf[0], o[i], 0, 0, 0);
       o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_h(vr[i][2], vr[i][3]), pf[1], o[i], 0, 0, 0);
     }
     if (more) load_v(st + kBaWaves);
-  }
+  };
+  for (const int plain = holes ? 0 : n >> 6; st < plain; st += kBaWaves) step(std::false_type());
+  for (; st < steps; st += kBaWaves) step(std::true_type());
   // the four waves' parts
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
@@ -336,17 +378,15 @@ __global__ __launch_bounds__(kJoinThreads) void k_blk_step_join(BlkAttn p) {
 }
 
 // ---------------------------------------------------------------- several rows a sequence
-// A tile is up to 32 CT columns (row, head of the KV head) of one sequence, rows outermost; a workgroup takes one tile
-// (and `chunk` of its keys where few rows meet long caches), its four waves every fourth 32 keys, 32 x 32 x 16 MFMA.
-// Each wave converts the codes it loads by itself and uses them for all CT 32 columns: no barrier stands in the loop,
-// and the q fragments, which the waves share, come from LDS.
-template <class E, int HD, int CT> struct RowsLds {
-  static constexpr int NP = Pieces<E>::kN, KU = HD / 32;
-  static constexpr int kQ = KU * 2 * NP * CT * 64 * 16;              // q fragments, 16 bytes a lane
-  static constexpr int kO = kBaWaves * CT * 32 * 33 * 4;             // 32 channels of every wave's sums (33: no bank conflicts)
-  static constexpr int kBytes = kQ > kO ? kQ : kO;
-};
-
+// A tile is up to `cols` columns (row, head of the KV head) of one sequence, rows outermost; a workgroup takes one tile (and
+// `chunk` of its keys where few rows meet long caches). 32 x 32 x 16 MFMA.
+//
+// k_blk_few: 32 columns. The four waves take every fourth 32 keys, each loading and converting its codes by itself: nothing
+// is shared but the columns, and no barrier stands in the loop.
+// k_blk_tile: 32 CT CG columns, CG groups of 32 CT for the waves; KG = 4 / CG waves of a group take the stage's 32 KG keys.
+// The workgroup loads a stage's codes together (a stage ahead), converts them once into LDS, in the MFMA operands' order,
+// two stages in turn with one barrier each. The conversion is as much vector work as the softmax of 32 columns (160
+// instructions of 32 keys at head dim 128 against 180), so CG waves share it.
 struct Tile {
   Seq s;
   int t, i0, rows;          // tile t of sequence s: its rows i0 .. i0 + rows - 1
@@ -354,273 +394,444 @@ struct Tile {
 };
 T2R_DEV bool find_tile(const BlkAttn& p, int cols, int w, Tile* t) {
   const int rt = cols / p.G;
-  t->t = find_piece(p.g, w, true, [&](const Seq& q) { return (q.n + rt - 1) / rt; }, &t->s);
+  t->t = find_piece(p.g, w, p.order, [&](const Seq& q) { return (q.n + rt - 1) / rt; }, &t->s);
   if (t->t < 0) return false;
   t->i0 = t->t * rt;
   t->rows = min(rt, t->s.n - t->i0);
   t->end = min(t->s.p0 + t->i0 + t->rows, (long long)p.c.width << p.c.lbs);
   return true;
 }
+// where column cc of a tile reads and writes
+T2R_DEV long long col_at(const Tile& t, int G, int hd, int kvh, int cc, long long ld) {
+  const int r = cc / G;
+  return (t.s.r0 + t.i0 + r) * ld + (long long)(kvh * G + cc - r * G) * hd;
+}
 
-template <class E, int HD, int CT>
-__global__ __launch_bounds__(kBaThreads, CT == 2 && HD == 128 ? 1 : 2) void k_blk_rows(BlkAttn p) {
-  constexpr int NP = Pieces<E>::kN, KU = HD / 32, DT = HD / 32, COLS = 32 * CT;
-  __shared__ BaSeg sg;
-  __shared__ float s_m[kBaWaves][COLS], s_l[kBaWaves][COLS];
-  __shared__ __align__(16) char s_big[RowsLds<E, HD, CT>::kBytes];
-  __shared__ int s_exp[COLS];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, c2 = lane >> 5;
-  const int w_tile = blockIdx.x / p.c.Hk, kvh = blockIdx.x - w_tile * p.c.Hk, split = blockIdx.y;
-  const int hd = p.c.hd, lbs = p.c.lbs, bmask = (1 << lbs) - 1, G = p.G;
-  Tile t;
-  if (!find_tile(p, COLS, w_tile, &t)) return;
-  const long long k0 = p.nsplit > 1 ? (long long)split * p.chunk : 0;
-  const int ncol = t.rows * G;
-  if (k0 >= t.end) {
-    if (split == 0)                                        // every row of the tile stands below position 0
-      for (int i = tid; i < ncol * hd; i += kBaThreads) {
-        const int c = i / hd, r = c / G;
-        ((E*)p.out)[(t.s.r0 + t.i0 + r) * p.out_ld + (long long)(kvh * G + c - r * G) * hd + (i - c * hd)] = narrow<E>(fv(kQNaN));
-      }
-    return;
+// a lane's column of q: its channels 32 u + 16 (lane / 32) .. + 15 (those past hd repeat the first ones) ...
+template <class E, int KU>
+T2R_DEV void q_load(const E* q, int hd, float (*x)[16]) {
+  const int c2 = (threadIdx.x & 63) >> 5;
+#pragma unroll
+  for (int u = 0; u < KU; ++u) {
+    const int d = u * 32 + c2 * 16;
+    Row16<E>::load(q + (d < hd ? d : 0), x[u]);
   }
-  const long long kend = p.nsplit > 1 ? min(t.end, k0 + p.chunk) : t.end;
-  const long long tile = p.c.tile_bytes();
-  // q fragments into LDS: unit (column, 16 channels); a row's largest magnitude first
-  v8h_t* qs = (v8h_t*)s_big;
-  {
-    constexpr int per = HD / 16, cols_at_once = kBaThreads / per;
-    for (int cb = 0; cb < COLS; cb += cols_at_once) {
-      const int cc = cb + tid / per, d = (tid % per) * 16, r = cc / G;
-      const bool live = cc < ncol && d < hd;
-      float x[16], am = 0;
-      if (live) {
-        Row16<E>::load((const E*)p.q + (t.s.r0 + t.i0 + r) * p.q_ld + (long long)(kvh * G + cc - r * G) * hd + d, x);
-      } else {
+}
+// ... and as fp16 pieces (zero past hd), in the order of K's rows; returns 2^e of the power that was taken out
+template <class E, int KU>
+T2R_DEV float q_pieces(int hd, const float (*x)[16], v8h_t (*qf)[Pieces<E>::kN][2]) {
+  constexpr int NP = Pieces<E>::kN;
+  const int c2 = (threadIdx.x & 63) >> 5;
+  float am = 0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = 0;
-      }
+  for (int u = 0; u < KU; ++u)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) am = fmaxf(am, fabsf(x[i]));
+    for (int i = 0; i < 16; ++i) am = fmaxf(am, fabsf(x[u][i]));
+  am = fmaxf(am, __shfl_xor(am, 32));
+  const int e = row_exp(am);
 #pragma unroll
-      for (int o = 1; o < per; o <<= 1) am = fmaxf(am, __shfl_xor(am, o));
-      const int e = row_exp(am);
-      const float down = pow2i(-e);
-      v8h_t f[NP][2];
+  for (int u = 0; u < KU; ++u) {
+    const float down = u * 32 + c2 * 16 < hd ? pow2i(-e) : 0.0f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float y = held(x[i] * down);
-        const _Float16 h = (_Float16)y;
-        f[0][i >> 3][i & 7] = h;
-        if (NP == 2) f[NP - 1][i >> 3][i & 7] = (_Float16)(y - (float)h);
-      }
-      // channels 32 u + 16 c + 8 half of column cc: fragment [u][half][piece][cc / 32], lane 32 c + cc % 32
-      const int u = d >> 5, ln = ((d >> 4) & 1) * 32 + (cc & 31);
-      if (cc < COLS) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int q = 0; q < NP; ++q) qs[(((u * 2 + half) * NP + q) * CT + (cc >> 5)) * 64 + ln] = f[q][half];
-        if (d == 0) s_exp[cc] = e;
-      }
+    for (int i = 0; i < 16; ++i) {
+      const float y = held(x[u][i] * down);
+      const _Float16 h = (_Float16)y;
+      qf[u][0][i >> 3][i & 7] = h;
+      if (NP == 2) qf[u][NP - 1][i >> 3][i & 7] = (_Float16)__builtin_fmaf((float)h, -1.0f, y);
     }
   }
-  // the last key that a lane's columns see (columns past the tile's: none of it matters)
-  long long lim[CT];
+  return pow2i(e);
+}
+
+// The softmax of 32 keys' scores s for a lane's column: this lane's 16 keys are 16 (lane / 32) + r, `left` of them (below 16
+// only if EDGE) are seen. Raises m where needed (o and l with it) and leaves the probabilities' pieces.
+template <int NP, int DT, bool EDGE>
+T2R_DEV void soft32(v16f_t& s, float sk, float lw, float iw, int left, float& m, float& l, v16f_t* o, v8h_t (*pf)[2]) {
+  if constexpr (EDGE) {
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct) lim[ct] = t.s.p0 + t.i0 + min(ct * 32 + col, ncol - 1) / G;
-  const long long all_see = t.s.p0 + t.i0 + 1;              // keys below this are seen by every row
-  float m[CT], l[CT], sq[CT], vref = 0;
-  v16f_t o[CT][DT];
+    for (int r = 0; r < 16; ++r) s[r] = r < left ? s[r] : kNegInf;
+  }
+  float mx = fmaxf(s[0], s[1]);
+#pragma unroll
+  for (int r = 2; r < 16; r += 2) mx = fmaxf(fmaxf(mx, s[r]), s[r + 1]);
+  mx *= sk;
+  if (__any(mx > m + kSlack)) {
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    const float n = mx > m + kSlack ? mx : m;
+    const float al = n == m ? 1.0f : __builtin_amdgcn_exp2f(m - n);
+    m = n;
+    l *= al;
+#pragma unroll
+    for (int i = 0; i < DT; ++i) o[i] *= al;
+  }
+  const float add = lw + kLift - (m == kNegInf ? 0.0f : m);
+  float ls[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sk, add));
+    ls[r & 3] += w;
+    const _Float16 h = (_Float16)w;
+    pf[0][r >> 3][r & 7] = h;
+    if (NP == 2) pf[NP - 1][r >> 3][r & 7] = (_Float16)__builtin_fmaf((float)h, -1.0f, w);      // (one mixed-precision step)
+  }
+  l = __builtin_fmaf((ls[0] + ls[1]) + (ls[2] + ls[3]), iw, l);
+}
+
+// The end of a tile: its waves' sums (wave's column group cg of 32 CT, key group kg of KG) are joined through LDS (so: KG x COLS
+// rows of HD + 4 floats, which keeps 16-byte accesses free of bank conflicts) and written as the result or, of a part of the
+// keys, into the workspace.
+template <class E, int HD, int CT, int CG, int NW> struct TileEnd {
+  static constexpr int KG = NW / CG, COLS = 32 * CT * CG, LD = HD + 4, kBytes = KG * COLS * LD * 4;
+  struct Ml { float m[KG][COLS], l[KG][COLS], top[COLS], sum[COLS], inv[COLS]; };
+};
+// four values side by side, at any element's alignment
+template <class E> T2R_DEV void store4(E* p, v4f_t x) {
+  struct __attribute__((packed, aligned(sizeof(E)))) V { E e[4]; };
+  *(V*)p = V{{narrow<E>(x[0]), narrow<E>(x[1]), narrow<E>(x[2]), narrow<E>(x[3])}};
+}
+template <class E, int HD, int CT, int CG, int NW>
+T2R_DEV void tile_end(const BlkAttn& p, const Tile& t, int kvh, int split, bool whole, float vref, float* m, float* l,
+                      v16f_t (*o)[HD / 32], typename TileEnd<E, HD, CT, CG, NW>::Ml& ml, float* so) {
+  using T = TileEnd<E, HD, CT, CG, NW>;
+  constexpr int KG = T::KG, COLS = T::COLS, LD = T::LD, DT = HD / 32;
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_index(), col = lane & 31, c2 = lane >> 5;
+  const int cg = wave % CG, kg = wave / CG, hd = p.c.hd, G = p.G, ncol = t.rows * G;
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
-    m[ct] = kNegInf;
-    l[ct] = 0;
+    l[ct] += __shfl_xor(l[ct], 32);
+    if (c2 == 0) {
+      ml.m[kg][(cg * CT + ct) * 32 + col] = m[ct];
+      ml.l[kg][(cg * CT + ct) * 32 + col] = l[ct];
+    }
+  }
+  __syncthreads();
+  // a column's largest maximum over its key groups, and the sum about it
+  if (tid < COLS) {
+    float mm = ml.m[0][tid], ls = 0;
+#pragma unroll
+    for (int w = 1; w < KG; ++w) mm = fmaxf(mm, ml.m[w][tid]);
+    const float mu = mm == kNegInf ? 0.0f : mm;
+#pragma unroll
+    for (int w = 0; w < KG; ++w) ls += __builtin_amdgcn_exp2f(ml.m[w][tid] - mu) * ml.l[w][tid];
+    ml.top[tid] = mm;
+    ml.sum[tid] = ls;
+    ml.inv[tid] = t.s.p0 + t.i0 + min(tid, ncol - 1) / G < 0 ? fv(kQNaN) : ls == 0 ? 0.0f : 1.0f / ls;
+  }
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int cc = (cg * CT + ct) * 32 + col;
+    float mm = ml.m[0][cc];
+#pragma unroll
+    for (int w = 1; w < KG; ++w) mm = fmaxf(mm, ml.m[w][cc]);
+    const float f = __builtin_amdgcn_exp2f(m[ct] - (mm == kNegInf ? 0.0f : mm)) * vref;
 #pragma unroll
     for (int i = 0; i < DT; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) o[ct][i][r] = 0;
+      for (int r = 0; r < 16; r += 4)
+        *(v4f_t*)(so + (kg * COLS + cc) * LD + i * 32 + 2 * r + 4 * c2) =
+            v4f_t{o[ct][i][r] * f, o[ct][i][r + 1] * f, o[ct][i][r + 2] * f, o[ct][i][r + 3] * f};
   }
-  for (long long seg = k0; seg < kend; seg += kBaSeg) {
-    const int n = (int)min((long long)kBaSeg, kend - seg);
-    const float vmax = fmaxf(vref, seg_load(sg, p.c, t.s.b, kvh, seg, n));
-    const int steps = (n + 31) >> 5;
-    if ((n + 15) / 16 < steps * 2 && tid == 0) {
-      sg.tb[steps * 2 - 1] = -1;
-      sg.ks[steps * 2 - 1] = 0;
-      sg.vs[steps * 2 - 1] = 0;
+  __syncthreads();
+  // four channels a thread
+  constexpr int PER = HD / 4;
+  const int d = tid % PER * 4;
+  if (d >= hd) return;
+#pragma unroll 2
+  for (int cc = tid / PER; cc < ncol; cc += 64 * NW / PER) {
+    v4f_t x = *(const v4f_t*)(so + cc * LD + d);
+#pragma unroll
+    for (int w = 1; w < KG; ++w) x += *(const v4f_t*)(so + (w * COLS + cc) * LD + d);
+    if (whole) {
+      store4((E*)p.out + col_at(t, G, hd, kvh, cc, p.out_ld) + d, x * ml.inv[cc]);
+    } else {
+      const long long at = ((long long)blockIdx.x * COLS + cc) * p.nsplit + split;
+      *(v4f_t*)(p.ws_o + at * hd + d) = x;
+      if (d == 0) {
+        p.ws_ml[2 * at] = ml.top[cc];
+        p.ws_ml[2 * at + 1] = ml.sum[cc];
+      }
     }
-    __syncthreads();
-    if (seg == k0) {
+  }
+}
+
+// The tile of a workgroup and its keys [k0, kend), false where it has none (a tile whose rows all stand below position 0 is
+// answered here).
+template <class E>
+T2R_DEV bool tile_of(const BlkAttn& p, int cols, Tile* t, int* kvh, long long* k0, long long* kend) {
+  const int w = blockIdx.x / p.c.Hk;
+  *kvh = blockIdx.x - w * p.c.Hk;
+  if (!find_tile(p, cols, w, t)) return false;
+  *k0 = p.nsplit > 1 ? (long long)blockIdx.y * p.chunk : 0;
+  *kend = p.nsplit > 1 ? min(t->end, *k0 + p.chunk) : t->end;
+  if (*k0 < t->end) return true;
+  if (blockIdx.y == 0)
+    for (int i = threadIdx.x; i < t->rows * p.G * p.c.hd; i += blockDim.x) {
+      const int cc = i / p.c.hd;
+      ((E*)p.out)[col_at(*t, p.G, p.c.hd, *kvh, cc, p.out_ld) + (i - cc * p.c.hd)] = narrow<E>(fv(kQNaN));
+    }
+  return false;
+}
+
+// how many of the 16 keys from `from` on a row at position `at` sees, `seen` of them there
+T2R_DEV int keys_left(long long at, long long from, int seen) {
+  const long long room = at - from;
+  return room < 0 ? 0 : min(room > 15 ? 16 : (int)room + 1, seen);
+}
+// whole steps of `step` keys at a segment's start that every row sees all of
+T2R_DEV int plain_steps(long long all_see, long long seg, int n, int step, bool holes) {
+  return holes ? 0 : (int)max(min(all_see - seg, (long long)n), 0LL) / step;
+}
+
+template <class E, int HD>
+__global__ __launch_bounds__(kBaThreads, 2) void k_blk_few(BlkAttn p) {
+  constexpr int NP = Pieces<E>::kN, KU = HD / 32, DT = HD / 32;
+  __shared__ BaSeg sg;
+  using End = TileEnd<E, HD, 1, 1, kBaWaves>;
+  __shared__ typename End::Ml ml;
+  __shared__ __align__(16) char s_o[End::kBytes];
+  const int lane = threadIdx.x & 63, wave = wave_index(), col = lane & 31, c2 = lane >> 5;
+  const int hd = p.c.hd, lbs = p.c.lbs, bmask = (1 << lbs) - 1, G = p.G;
+  Tile t;
+  int kvh;
+  long long k0, kend;
+  if (!tile_of<E>(p, 32, &t, &kvh, &k0, &kend)) return;
+  const int cc = min(col, t.rows * G - 1);
+  int blk = seg_table(p.c, t.s.b, k0, (int)min((long long)kBaSeg, kend - k0));
+  float x[KU][16];
+  q_load<E, KU>((const E*)p.q + col_at(t, G, hd, kvh, cc, p.q_ld), hd, x);
+  v8h_t qf[KU][NP][2];
+  const long long at = t.s.p0 + t.i0 + cc / G, all_see = t.s.p0 + t.i0 + 1;   // (keys below all_see are seen by every row)
+  const int tile = p.c.tile_bytes();
+  // row 8 i + 4 c' + r of the 32 stands for key 16 c' + 4 i + r
+  const int kc = (col >> 2) & 1, krow = 4 * (col >> 3) + (col & 3);
+  float m = kNegInf, l = 0, vref = 0;
+  v16f_t o[1][DT];
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) sq[ct] = p.a * pow2i(s_exp[ct * 32 + col]);
-    } else if (vmax > vref) {
-      const float f = vref / vmax;
+  for (int i = 0; i < DT; ++i) o[0][i] = v16f_t{};
+  v4i_t kr[KU], vr[DT];
+  auto load_k = [&](int st) {
+    const int ch = st * 2 + kc;
+    const int8_t* base = p.c.kc + (long long)sg.tb[ch] * tile + (((ch * 16) & bmask) + krow) * hd;
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
+    for (int u = 0; u < KU; ++u) {
+      const int d = u * 32 + c2 * 16;
+      kr[u] = *(const v4i_t*)(base + (d < hd ? d : 0));              // (past hd q is zero)
+    }
+  };
+  auto load_v = [&](int st) {
+    const int ch = st * 2 + c2;
+    const int8_t* base = p.c.vc + (long long)sg.tb[ch] * tile + ((ch * 16) & bmask);
 #pragma unroll
-        for (int i = 0; i < DT; ++i) o[ct][i] *= f;
+    for (int i = 0; i < DT; ++i) vr[i] = *(const v4i_t*)(base + (min(i * 32 + col, hd - 1) << lbs));
+  };
+  // a segment's blocks, and its first loads
+  auto begin = [&](int n) {
+    seg_blocks(sg, p.c, blk, kvh, n, 32);
+    if (wave < (n + 31) >> 5) {
+      load_k(wave);
+      load_v(wave);
+    }
+  };
+  begin((int)min((long long)kBaSeg, kend - k0));
+  const float sq = p.a * q_pieces<E, KU>(hd, x, qf);
+  for (long long seg = k0; seg < kend; seg += kBaSeg) {
+    const int n = (int)min((long long)kBaSeg, kend - seg), steps = (n + 31) >> 5;
+    bool holes;
+    const float vmax = seg_scales<kBaWaves>(sg, p.c, blk, kvh, n, 32, vref, &holes);
+    if (vmax > vref) {
+#pragma unroll
+      for (int i = 0; i < DT; ++i) o[0][i] *= vref / vmax;
     }
     vref = vmax;
-    v4i_t kr[KU], vr[DT];
-    // row 8 i + 4 c' + r of the 32 stands for key 16 c' + 4 i + r
-    const int kc = (col >> 2) & 1, krow = 4 * (col >> 3) + (col & 3);
-    auto load_k = [&](int st) {
-      const int ch = st * 2 + kc, tb = max(sg.tb[ch], 0);
-      const int8_t* base = p.c.kc + tb * tile + (long long)(((ch * 16) & bmask) + krow) * hd;
-#pragma unroll
-      for (int u = 0; u < KU; ++u) {
-        const int d = u * 32 + c2 * 16;
-        kr[u] = *(const v4i_t*)(base + (d < hd ? d : 0));
-      }
-    };
-    auto load_v = [&](int st) {
-      const int ch = st * 2 + c2, tb = max(sg.tb[ch], 0);
-      const int8_t* base = p.c.vc + tb * tile + ((ch * 16) & bmask);
-#pragma unroll
-      for (int i = 0; i < DT; ++i) vr[i] = *(const v4i_t*)(base + ((long long)min(i * 32 + col, hd - 1) << lbs));
-    };
     int st = wave;
-    if (st < steps) {
-      load_k(st);
-      load_v(st);
-    }
-    for (; st < steps; st += kBaWaves) {
-      v16f_t s[CT];
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[ct][r] = 0;
+    auto step = [&](auto edge) {
+      v16f_t s = {};
 #pragma unroll
       for (int u = 0; u < KU; ++u)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const v8h_t kf = codes_h(kr[u][2 * half], kr[u][2 * half + 1]);
 #pragma unroll
-          for (int q = 0; q < NP; ++q)
-#pragma unroll
-            for (int ct = 0; ct < CT; ++ct)
-              s[ct] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qs[(((u * 2 + half) * NP + q) * CT + ct) * 64 + lane], s[ct], 0, 0, 0);
+          for (int q = 0; q < NP; ++q) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[u][q][half], s, 0, 0, 0);
         }
       const bool more = st + kBaWaves < steps;
       if (more) load_k(st + kBaWaves);
       const int ch = st * 2 + c2;
-      const bool gone = sg.tb[ch] < 0;
-      const float ksc = sg.ks[ch];
-      float wv = 0;
-      if (vref > 0) wv = sg.vs[ch] / vref;
-      const bool edge = seg + st * 32 + 32 > all_see || __any(gone);
-      v8h_t pf[CT][NP][2];
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        const float sk = score_scale(sq[ct], ksc);
-        if (edge) {
-          // this lane's keys: seg + 32 st + 16 c2 + r
-          const long long room = lim[ct] - (seg + ch * 16);
-          const int left = gone || room < 0 ? 0 : room > 15 ? 16 : (int)room + 1;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[ct][r] = r < left ? s[ct][r] : kNegInf;
-        }
-        float mx = s[ct][0];
-#pragma unroll
-        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[ct][r]);
-        mx *= sk;
-        if (__any(mx > m[ct] + kSlack)) {
-          mx = fmaxf(mx, __shfl_xor(mx, 32));
-          if (mx > m[ct] + kSlack) {
-            const float al = __builtin_amdgcn_exp2f(m[ct] - mx);
-            m[ct] = mx;
-            l[ct] *= al;
-#pragma unroll
-            for (int i = 0; i < DT; ++i) o[ct][i] *= al;
-          }
-        }
-        const float sub = (m[ct] == kNegInf ? 0.0f : m[ct]) - kLift;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ct][r], sk, -sub));
-          l[ct] += e;
-          const float w = NP == 2 ? held(e * wv) : e * wv;
-          const _Float16 h = (_Float16)w;
-          pf[ct][0][r >> 3][r & 7] = h;
-          if (NP == 2) pf[ct][NP - 1][r >> 3][r & 7] = (_Float16)(w - (float)h);
-        }
-      }
+      v8h_t pf[NP][2];
+      soft32<NP, DT, edge.value>(s, score_scale(sq, sg.ks[ch]), sg.lw[ch], sg.iw[ch],
+                                 edge.value ? keys_left(at, seg + ch * 16, sg.seen[ch]) : 16, m, l, o[0], pf);
 #pragma unroll
       for (int i = 0; i < DT; ++i)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const v8h_t vf = codes_h(vr[i][2 * half], vr[i][2 * half + 1]);
 #pragma unroll
-          for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-            for (int q = 0; q < NP; ++q) o[ct][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[ct][q][half], o[ct][i], 0, 0, 0);
+          for (int q = 0; q < NP; ++q) o[0][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[q][half], o[0][i], 0, 0, 0);
         }
       if (more) load_v(st + kBaWaves);
+    };
+    for (const int plain = plain_steps(all_see, seg, n, 32, holes); st < plain; st += kBaWaves) step(std::false_type());
+    for (; st < steps; st += kBaWaves) step(std::true_type());
+    __syncthreads();                                        // the next segment's tables take this one's place
+    const long long next = seg + kBaSeg;
+    if (next < kend) {
+      const int m = (int)min((long long)kBaSeg, kend - next);
+      blk = seg_table(p.c, t.s.b, next, m);
+      begin(m);
     }
-    __syncthreads();                                        // the next segment's tables, or the sums below, reuse the LDS
   }
-  // the four waves' parts, 32 channels at a time
+  tile_end<E, HD, 1, 1, kBaWaves>(p, t, kvh, blockIdx.y, k0 == 0 && kend == t.end, vref, &m, &l, o, ml, (float*)s_o);
+}
+
+// LDS of k_blk_tile, in 16-byte slots: a fragment (64 lanes' operand of one MFMA) is 64 slots. K's fragments of a stage are
+// [kg][u][half], V's [kg][i][half]. The lane's slot is turned by the fragment's place, so that the loading threads, which
+// hold neighbouring 16-byte pieces of a token or channel, write to different banks.
+template <class E, int HD, int CT, int CG, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void k_blk_tile(BlkAttn p) {
+  constexpr int NP = Pieces<E>::kN, KU = HD / 32, DT = HD / 32, KG = NW / CG, COLS = 32 * CT * CG, THREADS = 64 * NW;
+  constexpr int STAGE = 32 * KG, FR = KG * KU * 2, PIECES = STAGE * HD / 16, PER = 2 * PIECES / THREADS;   // 16-byte pieces of K (as many of V)
+  using End = TileEnd<E, HD, CT, CG, NW>;
+  constexpr int kBufs = 2 * 2 * FR * 1024;
+  static_assert(PER * THREADS == 2 * PIECES && PIECES % 64 == 0, "whole loads");
+  __shared__ BaSeg sg;
+  __shared__ typename End::Ml ml;
+  __shared__ __align__(16) char s_big[kBufs > End::kBytes ? kBufs : End::kBytes];
+  v8h_t* bufs = (v8h_t*)s_big;
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_index(), col = lane & 31, c2 = lane >> 5;
+  const int cg = wave % CG, kg = wave / CG;
+  const int hd = p.c.hd, lbs = p.c.lbs, bmask = (1 << lbs) - 1, G = p.G;
+  Tile t;
+  int kvh;
+  long long k0, kend;
+  if (!tile_of<E>(p, COLS, &t, &kvh, &k0, &kend)) return;
+  const int ncol = t.rows * G;
+  int blk = seg_table(p.c, t.s.b, k0, (int)min((long long)kBaSeg, kend - k0));
+  v8h_t qf[CT][KU][NP][2];
+  float x[CT][KU][16], sq[CT], m[CT], l[CT], vref = 0;
+  long long at[CT];
+  v16f_t o[CT][DT];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
-    l[ct] += __shfl_xor(l[ct], 32);
-    if (c2 == 0) {
-      s_m[wave][ct * 32 + col] = m[ct];
-      s_l[wave][ct * 32 + col] = l[ct];
-    }
+    const int cc = min((cg * CT + ct) * 32 + col, ncol - 1);
+    q_load<E, KU>((const E*)p.q + col_at(t, G, hd, kvh, cc, p.q_ld), hd, x[ct]);
+    at[ct] = t.s.p0 + t.i0 + cc / G;
+    m[ct] = kNegInf;
+    l[ct] = 0;
+#pragma unroll
+    for (int i = 0; i < DT; ++i) o[ct][i] = v16f_t{};
   }
-  __syncthreads();
-  float f[CT];
+  const long long all_see = t.s.p0 + t.i0 + 1;                // keys below this are seen by every row
+  const int tile = p.c.tile_bytes();
+  v4i_t raw[PER];
+  // Piece j: of K token j / (HD / 16), channels 16 (j % (HD / 16)); past K's, of V channel j / (2 KG), tokens 16 (j % (2 KG)).
+  // (Which of them a wave's i-th is does not depend on the lane.)
+  auto of_v = [&](int i) { return PIECES % THREADS == 0 ? i >= PIECES / THREADS : wave * 64 + i * THREADS >= PIECES; };
+  auto load = [&](int st) {
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    float mm = kNegInf;
-#pragma unroll
-    for (int w = 0; w < kBaWaves; ++w) mm = fmaxf(mm, s_m[w][ct * 32 + col]);
-    f[ct] = __builtin_amdgcn_exp2f(m[ct] - (mm == kNegInf ? 0.0f : mm)) * vref;
-  }
-  const bool whole = k0 == 0 && kend == t.end;
-  float* so = (float*)s_big;
-#pragma unroll
-  for (int i = 0; i < DT; ++i) {
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        so[(wave * COLS + ct * 32 + col) * 33 + 8 * (r >> 2) + 4 * c2 + (r & 3)] = o[ct][i][r] * f[ct];
-    __syncthreads();
-    for (int e = tid; e < ncol * 32; e += kBaThreads) {
-      const int cc = e >> 5, d = i * 32 + (e & 31);
-      if (d >= hd) continue;
-      float x = 0, ls = 0, mm = kNegInf;
-#pragma unroll
-      for (int w = 0; w < kBaWaves; ++w) mm = fmaxf(mm, s_m[w][cc]);
-      const float mu = mm == kNegInf ? 0.0f : mm;
-#pragma unroll
-      for (int w = 0; w < kBaWaves; ++w) {
-        x += so[(w * COLS + cc) * 33 + (e & 31)];
-        ls += __builtin_amdgcn_exp2f(s_m[w][cc] - mu) * s_l[w][cc];
-      }
-      if (whole) {
-        const int r = cc / G;
-        ((E*)p.out)[(t.s.r0 + t.i0 + r) * p.out_ld + (long long)(kvh * G + cc - r * G) * hd + d] =
-            narrow<E>(t.s.p0 + t.i0 + r < 0 ? fv(kQNaN) : ls == 0 ? 0.0f : x / ls);
+    for (int i = 0; i < PER; ++i) {
+      const int j = tid + i * THREADS;
+      if (!of_v(i)) {
+        const int key = st * STAGE + j / (HD / 16), d = j % (HD / 16) * 16;
+        raw[i] = *(const v4i_t*)(p.c.kc + (long long)sg.tb[key >> 4] * tile + ((key & bmask) * hd + (d < hd ? d : 0)));
       } else {
-        const long long at = ((long long)blockIdx.x * COLS + cc) * p.nsplit + split;
-        p.ws_o[at * hd + d] = x;
-        if (d == 0) {
-          p.ws_ml[2 * at] = mm;
-          p.ws_ml[2 * at + 1] = ls;
-        }
+        const int jv = j - PIECES, ch = st * 2 * KG + jv % (2 * KG), d = jv / (2 * KG);
+        raw[i] = *(const v4i_t*)(p.c.vc + (long long)sg.tb[ch] * tile + (((ch * 16) & bmask) + (min(d, hd - 1) << lbs)));
       }
     }
-    __syncthreads();
+  };
+  auto put = [&](v8h_t* buf) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int j = tid + i * THREADS;
+      int fr, slot;
+      if (!of_v(i)) {
+        const int key = j / (HD / 16), dc = j % (HD / 16), k16 = key & 15;
+        fr = (key >> 5) * KU * 2 + (dc >> 1) * 2;
+        slot = ((dc & 1) * 32 + 8 * (k16 >> 2) + 4 * (key >> 4 & 1) + (k16 & 3)) ^ (dc & 7);    // (the token's row of the 32)
+      } else {
+        const int jv = j - PIECES, ck = jv % (2 * KG), d = jv / (2 * KG);
+        fr = FR + (ck >> 1) * DT * 2 + (d >> 5) * 2;
+        slot = ((ck & 1) * 32 + (d & 31)) ^ (2 * ck & 7);
+      }
+      buf[fr * 64 + slot] = codes_h(raw[i][0], raw[i][1]);
+      buf[(fr + 1) * 64 + slot] = codes_h(raw[i][2], raw[i][3]);
+    }
+  };
+  // a segment's blocks, and its first loads
+  auto begin = [&](int n) {
+    seg_blocks(sg, p.c, blk, kvh, n, STAGE);
+    load(0);
+  };
+  begin((int)min((long long)kBaSeg, kend - k0));
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) sq[ct] = p.a * q_pieces<E, KU>(hd, x[ct], qf[ct]);
+  for (long long seg = k0; seg < kend; seg += kBaSeg) {
+    const int n = (int)min((long long)kBaSeg, kend - seg), stages = (n + STAGE - 1) / STAGE;
+    bool holes;
+    const float vmax = seg_scales<NW>(sg, p.c, blk, kvh, n, STAGE, vref, &holes);
+    if (vmax > vref) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int i = 0; i < DT; ++i) o[ct][i] *= vref / vmax;
+    }
+    vref = vmax;
+    auto stage = [&](int st, auto edge) {
+      v8h_t* buf = bufs + (st & 1) * 2 * FR * 64;
+      put(buf);
+      __syncthreads();                                        // (the stage before last, in this buffer, is read: all were past it here)
+      if (st + 1 < stages) load(st + 1);
+      const int key0 = st * STAGE + kg * 32, ch = (key0 >> 4) + c2;
+      if (key0 >= n) return;
+      v16f_t s[CT];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) s[ct] = v16f_t{};
+#pragma unroll
+      for (int u = 0; u < KU; ++u)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const v8h_t kf = buf[((kg * KU + u) * 2 + half) * 64 + (lane ^ ((2 * u + c2) & 7))];
+#pragma unroll
+          for (int q = 0; q < NP; ++q)
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) s[ct] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[ct][u][q][half], s[ct], 0, 0, 0);
+        }
+      const float ks = sg.ks[ch], lw = sg.lw[ch], iw = sg.iw[ch];
+      const int seen = edge.value ? sg.seen[ch] : 16;
+      v8h_t pf[CT][NP][2];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+        soft32<NP, DT, edge.value>(s[ct], score_scale(sq[ct], ks), lw, iw, edge.value ? keys_left(at[ct], seg + ch * 16, seen) : 16,
+                                   m[ct], l[ct], o[ct], pf[ct]);
+#pragma unroll
+      for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const v8h_t vf = buf[(FR + (kg * DT + i) * 2 + half) * 64 + (lane ^ (2 * (2 * kg + c2) & 7))];
+#pragma unroll
+          for (int q = 0; q < NP; ++q)
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) o[ct][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[ct][q][half], o[ct][i], 0, 0, 0);
+        }
+    };
+    const int plain = plain_steps(all_see, seg, n, STAGE, holes);
+    int st = 0;
+    for (; st < plain; ++st) stage(st, std::false_type());
+    for (; st < stages; ++st) stage(st, std::true_type());
+    __syncthreads();                                          // the next segment's tables and stages, or the sums, take their place
+    const long long next = seg + kBaSeg;
+    if (next < kend) {
+      const int m2 = (int)min((long long)kBaSeg, kend - next);
+      blk = seg_table(p.c, t.s.b, next, m2);
+      begin(m2);
+    }
   }
+  tile_end<E, HD, CT, CG, NW>(p, t, kvh, blockIdx.y, k0 == 0 && kend == t.end, vref, m, l, o, ml, (float*)s_big);
 }
 
 // Joins the parts of a tile's columns: a workgroup per (KV head, tile, 4 columns)
-template <class E, int CT>
-__global__ __launch_bounds__(kBaThreads) void k_blk_rows_join(BlkAttn p) {
-  constexpr int COLS = 32 * CT;
+template <class E>
+__global__ __launch_bounds__(kBaThreads) void k_blk_rows_join(BlkAttn p, int COLS) {
   const int w_tile = blockIdx.x / p.c.Hk, kvh = blockIdx.x - w_tile * p.c.Hk;
   Tile t;
   if (!find_tile(p, COLS, w_tile, &t) || t.end <= p.chunk) return;

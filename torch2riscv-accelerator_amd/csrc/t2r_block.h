@@ -80,7 +80,7 @@ struct BlkCache {
   const int32_t* table;     // [B, width], rows `width` apart
   int n_blocks, Hk, hd, lbs, width;   // lbs = log2(bs)
   T2R_DEV int bs() const { return 1 << lbs; }
-  T2R_DEV long long tile_bytes() const { return (long long)hd << lbs; }
+  T2R_DEV int tile_bytes() const { return hd << lbs; }
   // the pool's block of sequence b's j-th one; -1 where the table has none (outside it, or an entry outside the pool)
   T2R_DEV int block(int b, long long j) const {
     if (j < 0 || j >= width) return -1;
@@ -110,45 +110,79 @@ T2R_DEV Seq seq_of(const Ragged& g, int b) {
   return s;
 }
 
-// The piece'th of all sequences' pieces, a sequence having count(Seq) of them, in order (backwards: from the last one).
-// Every wave of a workgroup finds it by itself, 64 sequences a step. Returns the piece's place in its sequence, -1 past
+// The piece'th of all sequences' pieces, a sequence having count(Seq) of them; in order, from the last one backwards, or the
+// later half backwards and then the earlier half forwards (a workgroup of the second round then does what its place in the
+// first left over, where pieces grow evenly: the tiles of a long prompt). Every wave of a workgroup finds it by itself, 64 sequences a step. Returns the piece's place in its sequence, -1 past
 // the last one.
+enum { ORDER_FORWARDS = 0, ORDER_BACKWARDS = 1, ORDER_BOTH = 2 };
+template <int CTRL, int ROWS = 0xF> T2R_DEV int dpp_or_0(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false); }
+// sums over lanes 0 .. lane; the largest of a wave's lanes' values (none below 0), in every lane
+T2R_DEV int wave_scan(int x) {
+  x += dpp_or_0<0x111>(x);                    // from 1, 2, 4, 8 lanes before, within 16
+  x += dpp_or_0<0x112>(x);
+  x += dpp_or_0<0x114>(x);
+  x += dpp_or_0<0x118>(x);
+  x += dpp_or_0<0x142, 0xA>(x);               // the last of the 16 before, then of the 32 before
+  return x + dpp_or_0<0x143, 0xC>(x);
+}
+T2R_DEV float wave_max0(float v) {
+  auto up = [&](int y) { v = fmaxf(v, fv((uint32_t)y)); };
+  up(dpp_or_0<0x111>((int)fb(v)));
+  up(dpp_or_0<0x112>((int)fb(v)));
+  up(dpp_or_0<0x114>((int)fb(v)));
+  up(dpp_or_0<0x118>((int)fb(v)));
+  up(dpp_or_0<0x142, 0xA>((int)fb(v)));
+  up(dpp_or_0<0x143, 0xC>((int)fb(v)));
+  return fv((uint32_t)__builtin_amdgcn_readlane((int)fb(v), 63));
+}
+
 template <class F>
-T2R_DEV int find_piece(const Ragged& g, int piece, bool backwards, F count, Seq* out) {
+T2R_DEV int find_piece(const Ragged& g, int piece, int order, F count, Seq* out) {
+  auto turn = [&](int total) {
+    if (order == ORDER_FORWARDS) return piece;
+    if (piece >= total) return -1;
+    const int half = order == ORDER_BOTH ? (total + 1) / 2 : total;
+    return piece < half ? total - 1 - piece : piece - half;
+  };
+  if (g.B == 1) {
+    *out = seq_of(g, 0);
+    const int total = count(*out), t = turn(total);
+    return t < total ? t : -1;
+  }
   const int lane = threadIdx.x & 63;
-  auto scan = [&](int b0, int* n, int* incl) {
+  Seq q;
+  int c, s;
+  auto scan = [&](int b0) {                   // 64 sequences: each lane's, its pieces, and the sum up to it
     const int b = b0 + lane;
-    int c = 0;
-    if (b < g.B) c = count(seq_of(g, b));
-    int s = c;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int t = __shfl_up(s, o);
-      s += lane >= o ? t : 0;
-    }
-    *n = c;
-    *incl = s;
+    q = seq_of(g, min(b, g.B - 1));
+    c = b < g.B ? count(q) : 0;
+    s = wave_scan(c);
     return __builtin_amdgcn_readlane(s, 63);
   };
-  int c, s;
-  if (backwards) {
-    int total = 0;
-    for (int b0 = 0; b0 < g.B; b0 += 64) total += scan(b0, &c, &s);
-    piece = total - 1 - piece;
+  int total = scan(0);
+  if (order != ORDER_FORWARDS) {
+    int sum = total;
+    for (int b0 = 64; b0 < g.B; b0 += 64) sum += scan(b0);
+    piece = turn(sum);
     if (piece < 0) return -1;
+    if (g.B > 64) total = scan(0);
   }
   int base = 0;
-  for (int b0 = 0; b0 < g.B; b0 += 64) {
-    const int total = scan(b0, &c, &s);
+  for (int b0 = 0;;) {
     if (piece < base + total) {
       const int l = __builtin_ctzll(__ballot(base + s > piece));
-      const int before = base + __builtin_amdgcn_readlane(s, l) - __builtin_amdgcn_readlane(c, l);
-      *out = seq_of(g, b0 + l);
-      return piece - before;
+      auto of = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
+      out->b = b0 + l;
+      out->r0 = of(q.r0);
+      out->n = of(q.n);
+      out->p0 = (long long)(((unsigned long long)(uint32_t)of((int)(q.p0 >> 32)) << 32) | (uint32_t)of((int)q.p0));
+      return piece - (base + of(s) - of(c));
     }
     base += total;
+    b0 += 64;
+    if (b0 >= g.B) return -1;
+    total = scan(b0);
   }
-  return -1;
 }
 
 // ---------------------------------------------------------------- rows into the cache, and out of it
@@ -195,7 +229,7 @@ __global__ __launch_bounds__(kBlkThreads) void k_blk_append(BlkRows x, Ragged g,
   const int tid = threadIdx.x, head = blockIdx.y, hd = c.hd, lbs = c.lbs;
   const bool is_v = blockIdx.z != 0;
   Seq s;
-  const int piece = find_piece(g, blockIdx.x, false, [&](const Seq& q) { return blocks_touched(q, lbs); }, &s);
+  const int piece = find_piece(g, blockIdx.x, ORDER_FORWARDS, [&](const Seq& q) { return blocks_touched(q, lbs); }, &s);
   if (piece < 0) return;
   const long long j = (s.p0 >> lbs) + piece, base = j << lbs;      // the sequence's j-th block, its first position
   const int blk = c.block(s.b, j);
@@ -276,7 +310,7 @@ __global__ __launch_bounds__(kBlkThreads) void k_blk_read(Ragged g, BlkCache c, 
   const int tid = threadIdx.x, head = blockIdx.y, hd = c.hd, lbs = c.lbs;
   const bool is_v = blockIdx.z != 0;
   Seq s;
-  const int piece = find_piece(g, blockIdx.x, false, [&](const Seq& q) { return blocks_touched(q, lbs); }, &s);
+  const int piece = find_piece(g, blockIdx.x, ORDER_FORWARDS, [&](const Seq& q) { return blocks_touched(q, lbs); }, &s);
   if (piece < 0) return;
   const long long j = (s.p0 >> lbs) + piece, base = j << lbs;
   const int blk = c.block(s.b, j);

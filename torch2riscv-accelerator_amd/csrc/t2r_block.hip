@@ -12,6 +12,10 @@
 
 using namespace t2r;
 
+#ifndef COLS64
+#define COLS64 (dtype != T2R_F32 ? 128 : 64)
+#define COLS128 64
+#endif
 namespace {
 
 inline int launched() { return hipGetLastError() == hipSuccess ? T2R_OK : T2R_EHIP; }
@@ -64,11 +68,12 @@ Cut step_cut(int B, int H, int Hk, int block, int width, int dtype) {
   c.nsplit = (int)cdiv(cap, c.chunk);
   return c;
 }
-Cut rows_cut(int B, int rows, int H, int Hk, int block, int width) {
+Cut rows_cut(int B, int rows, int H, int Hk, int hd, int block, int width, int dtype) {
   const long long cap = (long long)width * block;
   const int G = H / Hk;
   Cut c;
-  c.cols = (long long)rows * G <= 32LL * B ? 32 : 64;
+  // few rows: one tile of 32 columns a sequence; else 64, or 128 where a wave's registers hold two times 32 columns
+  c.cols = (long long)rows * G <= 32LL * B ? 32 : hd <= 64 ? COLS64 : COLS128;
   const int rt = c.cols / G;
   // every sequence's last tile may be a part of one
   const long long tiles = rows / rt + (B < rows ? B : rows);
@@ -141,7 +146,7 @@ int t2r_kv_read_blk(const int8_t* kc, const int8_t* vc, const float* ks, const f
 
 int64_t t2r_attn_blk_workspace_bytes(int B, int rows, int H, int Hk, int hd, int block, int width, int dtype) {
   if (B <= 0 || rows < 0 || !attn_shape_ok(H, Hk) || hd <= 0 || block <= 0 || width <= 0 || !dtype_ok(dtype)) return -1;
-  return rows == 0 ? step_ws(step_cut(B, H, Hk, block, width, dtype), B, H, hd) : rows_ws(rows_cut(B, rows, H, Hk, block, width), Hk, hd);
+  return rows == 0 ? step_ws(step_cut(B, H, Hk, block, width, dtype), B, H, hd) : rows_ws(rows_cut(B, rows, H, Hk, hd, block, width, dtype), Hk, hd);
 }
 
 int t2r_attn_blk_decode(const void* q, int dtype, int64_t q_ld, const int8_t* kc, const int8_t* vc, const float* ks,
@@ -186,7 +191,7 @@ int t2r_attn_blk_prefill(const void* q, int dtype, int64_t q_ld, const int8_t* k
   std::memset(&p, 0, sizeof(p));
   if (int rc = cache_args(kc, vc, ks, vs, n_blocks, block, Hk, hd, table, width, &p.c)) return rc;
   if (!attn_shape_ok(H, Hk) || B <= 0 || rows <= 0 || q_ld < (int64_t)H * hd || out_ld < (int64_t)H * hd) return T2R_ESHAPE;
-  const Cut cut = rows_cut(B, rows, H, Hk, block, width);
+  const Cut cut = rows_cut(B, rows, H, Hk, hd, block, width, dtype);
   if (cut.nsplit > 65535 || (long long)cut.tiles * Hk > INT32_MAX) return T2R_ESHAPE;
   const long long need = rows_ws(cut, Hk, hd);
   if (need > 0 && (!workspace || workspace_bytes < need || misaligned(workspace, 16))) return T2R_ENOMEM;
@@ -194,21 +199,28 @@ int t2r_attn_blk_prefill(const void* q, int dtype, int64_t q_ld, const int8_t* k
   p.g = Ragged{starts, lens, B, rows};
   p.H = H; p.G = H / Hk; p.a = scale * 1.44269504f;
   p.chunk = cut.chunk; p.nsplit = cut.nsplit;
+  p.order = (long long)cut.tiles * Hk <= 512 ? ORDER_BOTH : ORDER_BACKWARDS;
   p.ws_o = (float*)workspace;
   p.ws_ml = p.ws_o + (long long)cut.tiles * Hk * cut.cols * cut.nsplit * hd;
   const hipStream_t st = (hipStream_t)stream;
   return by_type(dtype, [&](auto e) {
     using E = decltype(e);
-    const dim3 grid(cut.tiles * Hk, cut.nsplit), jg(cut.tiles * Hk, cut.cols / 4);
+    const dim3 grid(cut.tiles * Hk, cut.nsplit), block(kBaThreads);
+    constexpr int CT = sizeof(E) == 2 ? 2 : 1;
     if (cut.cols == 32) {
-      if (hd <= 64) launch((k_blk_rows<E, 64, 1>), grid, dim3(kBaThreads), 0, st, p);
-      else launch((k_blk_rows<E, 128, 1>), grid, dim3(kBaThreads), 0, st, p);
-      if (cut.nsplit > 1) launch((k_blk_rows_join<E, 1>), jg, dim3(kBaThreads), 0, st, p);
+      if (hd <= 64) launch((k_blk_few<E, 64>), grid, block, 0, st, p);
+      else launch((k_blk_few<E, 128>), grid, block, 0, st, p);
     } else {
-      if (hd <= 64) launch((k_blk_rows<E, 64, 2>), grid, dim3(kBaThreads), 0, st, p);
-      else launch((k_blk_rows<E, 128, 2>), grid, dim3(kBaThreads), 0, st, p);
-      if (cut.nsplit > 1) launch((k_blk_rows_join<E, 2>), jg, dim3(kBaThreads), 0, st, p);
+#ifndef CFG64
+#define CFG64 CT, 2, 4
+#define CFG128 1, 2, 4
+#define NW64 4
+#define NW128 4
+#endif
+      if (hd <= 64) launch((k_blk_tile<E, 64, CFG64>), grid, dim3(64 * NW64), 0, st, p);
+      else launch((k_blk_tile<E, 128, CFG128>), grid, dim3(64 * NW128), 0, st, p);
     }
+    if (cut.nsplit > 1) launch(k_blk_rows_join<E>, dim3(cut.tiles * Hk, cut.cols / 4), block, 0, st, p, cut.cols);
     return launched();
   });
 }
