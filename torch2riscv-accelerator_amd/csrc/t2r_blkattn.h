@@ -149,14 +149,14 @@ T2R_DEV float seg_scales(BaSeg& sg, const BlkCache& c, int blk, int head, int n,
 template <class E> struct Pieces { static constexpr int kN = sizeof(E) == 4 ? 2 : 1, kHeads = 16 / kN; };
 
 template <class E, int HD>
-__global__ __launch_bounds__(kBaThreads) void k_blk_step(BlkAttn p) {
+__global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_step(BlkAttn p) {
   constexpr int NP = Pieces<E>::kN, HW = Pieces<E>::kHeads, KU = HD / 64, DT = HD / 16;
   __shared__ BaSeg sg;
   __shared__ float s_m[kBaWaves][16], s_l[kBaWaves][16];
   __shared__ float s_o[kBaWaves][16][HD + 4];
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_index(), col = lane & 15, c4 = lane >> 4;
   const int sets = (p.G + HW - 1) / HW;
-  const int kvh = blockIdx.x / sets, h0 = (blockIdx.x - kvh * sets) * HW, b = blockIdx.z, split = blockIdx.y;
+  const int kvh = blockIdx.x / sets, h0 = (blockIdx.x - kvh * sets) * HW, b = blockIdx.y, split = blockIdx.z;
   const int hd = p.c.hd, lbs = p.c.lbs, bmask = (1 << lbs) - 1;
   const int nh = min(HW, p.G - h0);                       // heads of this workgroup
   const long long k0 = (long long)split * p.chunk;
@@ -352,29 +352,67 @@ __global__ __launch_bounds__(kBaThreads) void k_blk_step(BlkAttn p) {
   }
 }
 
-// Joins the parts of a long row: a workgroup per (head, sequence).
-constexpr int kJoinThreads = 128;
-template <class E>
-T2R_DEV void join_row(const BlkAttn& p, long long at, int parts, E* out, int d, bool place) {
+// Joins the parts of a row: their sums, moved to the largest of their maxima. NWV waves take every NWV-th part each, a lane
+// two channels; what a wave has comes back in *x (and the weights' sum, the same in every wave). The parts' maxima are read
+// 64 at a time, a lane each; the sums' loads wait for nothing.
+template <int NWV>
+T2R_DEV float join_parts(const BlkAttn& p, long long at, int parts, int wave, float (*x)[2]) {
+  const int lane = threadIdx.x & 63, hd = p.c.hd, d = min(2 * lane, hd - 2);
+  typedef float v2f_t __attribute__((ext_vector_type(2)));
+  const v2f_t* ml = (const v2f_t*)p.ws_ml + at;
   float mm = kNegInf;
-  for (int s = 0; s < parts; ++s) mm = fmaxf(mm, p.ws_ml[2 * (at + s)]);
+  for (int s = lane; s < parts; s += 64) mm = fmaxf(mm, ml[s][0]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o));
   const float mu = mm == kNegInf ? 0.0f : mm;
-  float x = 0, l = 0;
+  float l = 0;
+  v2f_t y = {0, 0};
+  for (int b = 0; b < parts; b += 64) {
+    const int n = min(parts - b, 64);
+    v2f_t v = {kNegInf, 0};
+    if (lane < n) v = ml[b + lane];
+    const float f = __builtin_amdgcn_exp2f(v[0] - mu);
+    l += f * v[1];
+    const float* o = p.ws_o + (at + b) * hd + d;
 #pragma unroll 8
-  for (int s = 0; s < parts; ++s) {
-    const float f = __builtin_amdgcn_exp2f(p.ws_ml[2 * (at + s)] - mu);
-    x += f * p.ws_o[(at + s) * p.c.hd + d];
-    l += f * p.ws_ml[2 * (at + s) + 1];
+    for (int s = wave; s < n; s += NWV) y += fv((uint32_t)__builtin_amdgcn_readlane((int)fb(f), s)) * *(const v2f_t*)(o + s * hd);
   }
-  *out = narrow<E>(!place ? fv(kQNaN) : l == 0 ? 0.0f : x / l);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
+  (*x)[0] = y[0];
+  (*x)[1] = y[1];
+  return l;
 }
+// two channels of a joined row; place: it stands in its sequence
 template <class E>
-__global__ __launch_bounds__(kJoinThreads) void k_blk_step_join(BlkAttn p) {
-  const int h = blockIdx.x, b = blockIdx.y, d = threadIdx.x;
+T2R_DEV void join_store(const BlkAttn& p, E* out, const float* x, float l, bool place) {
+  const int d = 2 * (threadIdx.x & 63);
+  if (d >= p.c.hd) return;
+  const float inv = !place ? fv(kQNaN) : l == 0 ? 0.0f : 1.0f / l;
+  out[d] = narrow<E>(x[0] * inv);
+  out[d + 1] = narrow<E>(x[1] * inv);
+}
+
+// a workgroup per (head, sequence)
+template <class E>
+__global__ __launch_bounds__(kBaThreads) void k_blk_step_join(BlkAttn p) {
+  __shared__ float s_x[kBaWaves][64][2];
+  const int h = blockIdx.x, b = blockIdx.y, wave = wave_index(), lane = threadIdx.x & 63;
   const long long len = min((long long)p.g.lens[b], (long long)p.c.width << p.c.lbs);
-  if (len <= p.chunk || d >= p.c.hd) return;              // one part (or none): written already
+  if (len <= p.chunk) return;                             // one part (or none): written already
   const int parts = (int)((len + p.chunk - 1) / p.chunk);
-  join_row<E>(p, ((long long)b * p.H + h) * p.nsplit, parts, (E*)p.out + (long long)b * p.out_ld + (long long)h * p.c.hd + d, d, true);
+  float x[2];
+  const float l = join_parts<kBaWaves>(p, ((long long)b * p.H + h) * p.nsplit, parts, wave, &x);
+  s_x[wave][lane][0] = x[0];
+  s_x[wave][lane][1] = x[1];
+  __syncthreads();
+  if (wave > 0) return;
+#pragma unroll
+  for (int w = 1; w < kBaWaves; ++w) {
+    x[0] += s_x[w][lane][0];
+    x[1] += s_x[w][lane][1];
+  }
+  join_store<E>(p, (E*)p.out + (long long)b * p.out_ld + (long long)h * p.c.hd, x, l, true);
 }
 
 // ---------------------------------------------------------------- several rows a sequence
@@ -829,18 +867,18 @@ __global__ __launch_bounds__(64 * NW, 2) void k_blk_tile(BlkAttn p) {
   tile_end<E, HD, CT, CG, NW>(p, t, kvh, blockIdx.y, k0 == 0 && kend == t.end, vref, m, l, o, ml, (float*)s_big);
 }
 
-// Joins the parts of a tile's columns: a workgroup per (KV head, tile, 4 columns)
+// Joins the parts of a tile's columns: a wave a column
 template <class E>
-__global__ __launch_bounds__(kBaThreads) void k_blk_rows_join(BlkAttn p, int COLS) {
+__global__ __launch_bounds__(kBaThreads) void k_blk_rows_join(BlkAttn p, int cols) {
   const int w_tile = blockIdx.x / p.c.Hk, kvh = blockIdx.x - w_tile * p.c.Hk;
   Tile t;
-  if (!find_tile(p, COLS, w_tile, &t) || t.end <= p.chunk) return;
-  const int cc = blockIdx.y * 4 + (threadIdx.x >> 6), G = p.G;
-  if (cc >= t.rows * G) return;
-  const int parts = (int)((t.end + p.chunk - 1) / p.chunk), r = cc / G;
-  const long long at = ((long long)blockIdx.x * COLS + cc) * p.nsplit;
-  E* out = (E*)p.out + (t.s.r0 + t.i0 + r) * p.out_ld + (long long)(kvh * G + cc - r * G) * p.c.hd;
-  for (int d = threadIdx.x & 63; d < p.c.hd; d += 64) join_row<E>(p, at, parts, out + d, d, t.s.p0 + t.i0 + r >= 0);
+  if (!find_tile(p, cols, w_tile, &t) || t.end <= p.chunk) return;
+  const int cc = blockIdx.y * kBaWaves + wave_index();
+  if (cc >= t.rows * p.G) return;
+  const int parts = (int)((t.end + p.chunk - 1) / p.chunk);
+  float x[2];
+  const float l = join_parts<1>(p, ((long long)blockIdx.x * cols + cc) * p.nsplit, parts, 0, &x);
+  join_store<E>(p, (E*)p.out + col_at(t, p.G, p.c.hd, kvh, cc, p.out_ld), x, l, t.s.p0 + t.i0 + cc / p.G >= 0);
 }
 
 }  // namespace t2r

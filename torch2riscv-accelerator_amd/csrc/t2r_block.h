@@ -187,7 +187,6 @@ T2R_DEV int find_piece(const Ragged& g, int piece, int order, F count, Seq* out)
 
 // ---------------------------------------------------------------- rows into the cache, and out of it
 constexpr int kBlkThreads = 256;
-constexpr int kMaxBlkTokens = 128;
 
 // the blocks that a sequence's rows lie in (the places below position 0 and past the table among them)
 T2R_DEV int blocks_touched(const Seq& s, int lbs) {
@@ -220,10 +219,16 @@ struct BlkRows {
   long long k_ld, v_ld;     // elements from row to row
 };
 
+// bytes [from, to) of word i of 16 bytes, as a mask
+T2R_DEV uint32_t byte_mask(int i, int from, int to) {
+  const int a = min(max(from - 4 * i, 0), 4), b = min(max(to - 4 * i, 0), 4);
+  return (uint32_t)((1ull << (8 * b)) - (1ull << (8 * a)));
+}
+
 // Rows into the cache: a workgroup takes one (block, KV head) of K or of V that rows enter: their maximum, the block's
-// new scale, the codes, and the block's older codes where the scale grew. The rows pass through registers once
-// (4 x 16 values a thread hold a 128 x 128 tile).
-template <class E>
+// new scale, the codes, and the block's older codes where the scale grew. A thread has NU units of 16 values, which stay in
+// registers between the two: K (token, 16 channels), V (channel, 16 tokens: lanes along the channels).
+template <class E, int NU>
 __global__ __launch_bounds__(kBlkThreads) void k_blk_append(BlkRows x, Ragged g, BlkCache c) {
   __shared__ float red[kBlkThreads / 64];
   const int tid = threadIdx.x, head = blockIdx.y, hd = c.hd, lbs = c.lbs;
@@ -242,32 +247,23 @@ __global__ __launch_bounds__(kBlkThreads) void k_blk_append(BlkRows x, Ragged g,
   const long long ld = is_v ? x.v_ld : x.k_ld;
   const E* src = (const E*)(is_v ? x.v : x.k) + row * ld + (long long)head * hd;
   const float was = lo > 0 ? *scale : 0.0f;
-  // units of 16 values: K (slot, 16 channels), V (channel, 16 slots: lanes along the channels)
   const int per = is_v ? hd : hd >> 4, units = is_v ? per << (lbs - 4) : per << lbs;
-  float val[4][16];
+  float val[NU][16];
   float m = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int u = tid + i * kBlkThreads;
-    if (u >= units) break;
-    const int a = u / per, b = u - a * per;
+  for (int i = 0; i < NU; ++i) {
+    const int u = min(tid + i * kBlkThreads, units - 1), a = u / per, b = u - a * per;
+    // (what is no row of the call repeats one that is: its maximum counts anyway)
     if (is_v) {
 #pragma unroll
-      for (int t = 0; t < 16; ++t) {
-        const int slot = a * 16 + t;
-        val[i][t] = slot >= lo && slot < hi ? widen(src[slot * ld + b]) : 0.0f;
-      }
-    } else if (a >= lo && a < hi) {
-      Row16<E>::load(src + a * ld + b * 16, val[i]);
+      for (int t = 0; t < 16; ++t) val[i][t] = widen(src[min(max(a * 16 + t, lo), hi - 1) * ld + b]);
     } else {
-#pragma unroll
-      for (int t = 0; t < 16; ++t) val[i][t] = 0;
+      Row16<E>::load(src + min(max(a, lo), hi - 1) * ld + b * 16, val[i]);
     }
 #pragma unroll
     for (int t = 0; t < 16; ++t) m = fmaxf(m, fabsf(val[i][t]));      // (a NaN is left out)
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  m = wave_max0(m);
   if ((tid & 63) == 0) red[tid >> 6] = m;
   __syncthreads();
   m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
@@ -276,28 +272,43 @@ __global__ __launch_bounds__(kBlkThreads) void k_blk_append(BlkRows x, Ragged g,
   const bool grew = lo > 0 && now > was && was > 0;
   // small scales are worked with 2^64 times larger, which is exact, so that 1 / s exists
   const float up = now < 0x1p-64f ? 0x1p64f : 1.0f, sn = now * up, inv = now > 0 ? 1.0f / sn : 0.0f;
-  const float ratio = grew ? was / now : 1.0f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < NU; ++i) {
     const int u = tid + i * kBlkThreads;
     if (u >= units) break;
     const int a = u / per, b = u - a * per;
-    int8_t* dst = tile + (is_v ? ((long long)b << lbs) + a * 16 : (long long)a * hd + b * 16);
+    int8_t* dst = tile + (is_v ? (b << lbs) + a * 16 : a * hd + b * 16);
     const int n_old = is_v ? min(max(lo - a * 16, 0), 16) : a < lo ? 16 : 0;     // values [0, n_old) are older ones,
     const int n_end = is_v ? min(max(hi - a * 16, 0), 16) : a < hi ? 16 : 0;     // [n_old, n_end) new ones
     if (n_end == 0 || (n_old == n_end && !grew)) continue;
     v4i_t w = {0, 0, 0, 0};
     if (n_old > 0 || n_end < 16) w = *(const v4i_t*)dst;
+    if (grew && n_old > 0) {
+      const float ratio = was / now;
+      for (int t = 0; t < n_old; t += 4) {
+        // (a word of w by its index, four codes; rare, so short rather than fast)
+        const uint32_t o = (uint32_t)(t < 8 ? t < 4 ? w[0] : w[1] : t < 12 ? w[2] : w[3]);
+        uint32_t r = 0;
 #pragma unroll
-    for (int t = 0; t < 16; ++t) {
-      const int sh = 8 * (t & 3);
-      int q = (int8_t)(w[t >> 2] >> sh);
-      if (t < n_old) {
-        if (grew) q = requant_code(q, was, now, ratio);
-      } else if (t < n_end) {
-        q = now > 0 ? quant_code(val[i][t] * up, sn, inv) : 0;
+        for (int k = 0; k < 4; ++k) r |= (uint32_t)(requant_code((int8_t)(o >> (8 * k)), was, now, ratio) & 0xFF) << (8 * k);
+        const uint32_t keep = byte_mask(t >> 2, 0, n_old);
+        r = (r & keep) | (o & ~keep);
+        if (t == 0) w[0] = (int)r;
+        else if (t == 4) w[1] = (int)r;
+        else if (t == 8) w[2] = (int)r;
+        else w[3] = (int)r;
       }
-      w[t >> 2] = (w[t >> 2] & ~(0xFF << sh)) | ((q & 0xFF) << sh);
+    }
+    if (n_old < n_end) {
+#pragma unroll
+      for (int t = 0; t < 16; t += 4) {
+        uint32_t r = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          r |= (uint32_t)((now > 0 ? quant_code(val[i][t + k] * up, sn, inv) : 0) & 0xFF) << (8 * k);
+        const uint32_t put = byte_mask(t >> 2, n_old, n_end);
+        w[t >> 2] = (int)((r & put) | ((uint32_t)w[t >> 2] & ~put));
+      }
     }
     *(v4i_t*)dst = w;
   }
@@ -305,7 +316,7 @@ __global__ __launch_bounds__(kBlkThreads) void k_blk_append(BlkRows x, Ragged g,
 }
 
 // Rows out of the cache, as the values that the codes stand for; zeros where the table holds no such position.
-template <class E>
+template <class E, int NU>
 __global__ __launch_bounds__(kBlkThreads) void k_blk_read(Ragged g, BlkCache c, E* k, E* v) {
   const int tid = threadIdx.x, head = blockIdx.y, hd = c.hd, lbs = c.lbs;
   const bool is_v = blockIdx.z != 0;
@@ -322,14 +333,14 @@ __global__ __launch_bounds__(kBlkThreads) void k_blk_read(Ragged g, BlkCache c, 
   E* dst = (is_v ? v : k) + row * ld + (long long)head * hd;
   const int per = is_v ? hd : hd >> 4, units = is_v ? per << (lbs - 4) : per << lbs;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < NU; ++i) {
     const int u = tid + i * kBlkThreads;
     if (u >= units) break;
     const int a = u / per, b = u - a * per;
     const int from = is_v ? max(lo - a * 16, 0) : a >= lo ? 0 : 16, to = is_v ? min(hi - a * 16, 16) : a < hi ? 16 : 0;
     if (from >= to) continue;
     v4i_t w = {0, 0, 0, 0};
-    if (blk >= 0) w = *(const v4i_t*)(tile + (is_v ? ((long long)b << lbs) + a * 16 : (long long)a * hd + b * 16));
+    if (blk >= 0) w = *(const v4i_t*)(tile + (is_v ? (b << lbs) + a * 16 : a * hd + b * 16));
     float y[16];
 #pragma unroll
     for (int t = 0; t < 16; ++t) y[t] = (float)(int8_t)(w[t >> 2] >> (8 * (t & 3))) * scale;

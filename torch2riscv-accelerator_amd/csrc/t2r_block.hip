@@ -53,18 +53,30 @@ long long blocks_entered(long long rows, long long B, int block) {
   return s + (x < x / block + s ? x : x / block + s);
 }
 
-// How the step form is cut: `chunk` keys a workgroup, so that the launch has some thousand workgroups as long as a chunk
-// keeps its four waves one step of 64 keys each. The lengths are on the device: the table's width bounds them, and
+// units of 16 values that a thread of the append and read kernels has (1, 2 or 4): 128 x 128 values are the most
+int units_of(int hd, int block) {
+  const int n = hd * block;
+  return n <= 16 * kBlkThreads ? 1 : n <= 32 * kBlkThreads ? 2 : 4;
+}
+
+// How the step form is cut: `chunk` keys a workgroup. The lengths are on the device: the table's width bounds them, and
 // workgroups past a sequence's end return at once.
+//  - A cache that one workgroup gets through in some 10 us stays whole, which saves the join's launch (3.3 us on the GPU, 3
+//    on the host). One sequence of 32 heads of 64 in a 2048-token table: 96 / 700 / 2040 tokens 4.9 / 7.1 / 11.7 us (10.7 /
+//    10.7 / 11.9 a call) whole, 8.7 / 9.1 / 9.2 (13.6 .. 13.8) in parts; at head dim 128 2040 tokens take 17 us whole.
+//  - Otherwise some 2000 workgroups: fewer leave a ragged batch's longest sequences over at the end, more begin and end too
+//    often. 32 sequences of 1021 .. 8192 tokens, 16 heads of 128: 66.6 us, 68.5 with half as many, 75 with twice; all of 8192:
+//    98.8 us (5.4 TB/s), 96.7, 116.
 struct Cut {
   int chunk, nsplit, tiles, cols;       // tiles and their columns: the ragged form
 };
-Cut step_cut(int B, int H, int Hk, int block, int width, int dtype) {
+Cut step_cut(int B, int H, int Hk, int hd, int block, int width, int dtype) {
   const long long cap = (long long)width * block;
   const int heads = dtype == T2R_F32 ? 8 : 16, sets = (H / Hk + heads - 1) / heads;
   const long long units = (long long)B * Hk * sets;
+  const bool whole = cap * (hd <= 64 ? 64 : 128) <= 2048 * 64;
   Cut c{256, 1, 0, 0};
-  while (c.chunk < kBaSeg && units * cdiv(cap, c.chunk) > 2048) c.chunk *= 2;
+  while (c.chunk < kBaSeg && c.chunk < cap && (whole || units * cdiv(cap, c.chunk) > 2048)) c.chunk *= 2;
   c.nsplit = (int)cdiv(cap, c.chunk);
   return c;
 }
@@ -81,12 +93,13 @@ Cut rows_cut(int B, int rows, int H, int Hk, int hd, int block, int width, int d
   const long long wgs = tiles * Hk;
   c.chunk = (int)cap;
   c.nsplit = 1;
-  if (wgs < 512) {
-    const long long want = cdiv(1024, wgs);
-    long long ch = cdiv(cdiv(cap, want), 128) * 128;
-    if (ch < 256) ch = 256;
-    c.chunk = (int)ch;
-    c.nsplit = (int)cdiv(cap, ch);
+  // A part costs what a tile costs before and after its keys (7 us) and the join's launch (5 us); 64 keys of a tile take 1.3
+  // us. So keys are cut only while workgroups leave half of the chip's places empty, and into parts of 512 at least: a
+  // 1024-row prompt (256 workgroups) took 30 + 13 us in four parts and 31 whole, 8 rows at 8100 positions 200 us whole.
+  if (wgs <= 256) {
+    const long long want = 512 / wgs, ch = cdiv(cdiv(cap, want), 128) * 128;
+    c.chunk = (int)(ch < 512 ? 512 : ch);
+    c.nsplit = (int)cdiv(cap, c.chunk);
   }
   return c;
 }
@@ -122,7 +135,14 @@ int t2r_kv_append_blk(const void* k, const void* v, int dtype, int64_t k_ld, int
   const Ragged g{starts, lens, B, rows};
   const dim3 grid((unsigned)blocks_entered(rows, B, block), Hk, 2);
   return by_type(dtype, [&](auto e) {
-    launch(k_blk_append<decltype(e)>, grid, dim3(kBlkThreads), 0, (hipStream_t)stream, x, g, c);
+    using E = decltype(e);
+    const dim3 threads(kBlkThreads);
+    const hipStream_t st = (hipStream_t)stream;
+    switch (units_of(hd, block)) {
+      case 1: launch((k_blk_append<E, 1>), grid, threads, 0, st, x, g, c); break;
+      case 2: launch((k_blk_append<E, 2>), grid, threads, 0, st, x, g, c); break;
+      default: launch((k_blk_append<E, 4>), grid, threads, 0, st, x, g, c); break;
+    }
     return launched();
   });
 }
@@ -139,14 +159,20 @@ int t2r_kv_read_blk(const int8_t* kc, const int8_t* vc, const float* ks, const f
   const dim3 grid((unsigned)blocks_entered(rows, B, block), Hk, 2);
   return by_type(dtype, [&](auto e) {
     using E = decltype(e);
-    launch(k_blk_read<E>, grid, dim3(kBlkThreads), 0, (hipStream_t)stream, g, c, (E*)k, (E*)v);
+    const dim3 threads(kBlkThreads);
+    const hipStream_t st = (hipStream_t)stream;
+    switch (units_of(hd, block)) {
+      case 1: launch((k_blk_read<E, 1>), grid, threads, 0, st, g, c, (E*)k, (E*)v); break;
+      case 2: launch((k_blk_read<E, 2>), grid, threads, 0, st, g, c, (E*)k, (E*)v); break;
+      default: launch((k_blk_read<E, 4>), grid, threads, 0, st, g, c, (E*)k, (E*)v); break;
+    }
     return launched();
   });
 }
 
 int64_t t2r_attn_blk_workspace_bytes(int B, int rows, int H, int Hk, int hd, int block, int width, int dtype) {
   if (B <= 0 || rows < 0 || !attn_shape_ok(H, Hk) || hd <= 0 || block <= 0 || width <= 0 || !dtype_ok(dtype)) return -1;
-  return rows == 0 ? step_ws(step_cut(B, H, Hk, block, width, dtype), B, H, hd) : rows_ws(rows_cut(B, rows, H, Hk, hd, block, width, dtype), Hk, hd);
+  return rows == 0 ? step_ws(step_cut(B, H, Hk, hd, block, width, dtype), B, H, hd) : rows_ws(rows_cut(B, rows, H, Hk, hd, block, width, dtype), Hk, hd);
 }
 
 int t2r_attn_blk_decode(const void* q, int dtype, int64_t q_ld, const int8_t* kc, const int8_t* vc, const float* ks,
@@ -159,7 +185,7 @@ int t2r_attn_blk_decode(const void* q, int dtype, int64_t q_ld, const int8_t* kc
   std::memset(&p, 0, sizeof(p));
   if (int rc = cache_args(kc, vc, ks, vs, n_blocks, block, Hk, hd, table, width, &p.c)) return rc;
   if (!attn_shape_ok(H, Hk) || B <= 0 || B > 65535 || H > 65535 || q_ld < (int64_t)H * hd || out_ld < (int64_t)H * hd) return T2R_ESHAPE;
-  const Cut cut = step_cut(B, H, Hk, block, width, dtype);
+  const Cut cut = step_cut(B, H, Hk, hd, block, width, dtype);
   if (cut.nsplit > 65535) return T2R_ESHAPE;
   const long long need = step_ws(cut, B, H, hd);
   if (need > 0 && (!workspace || workspace_bytes < need || misaligned(workspace, 16))) return T2R_ENOMEM;
@@ -173,10 +199,11 @@ int t2r_attn_blk_decode(const void* q, int dtype, int64_t q_ld, const int8_t* kc
   return by_type(dtype, [&](auto e) {
     using E = decltype(e);
     const int sets = (p.G + Pieces<E>::kHeads - 1) / Pieces<E>::kHeads;
-    const dim3 grid(Hk * sets, cut.nsplit, B);
+    // later parts come last: those past their sequence's end, which return at once, then hold up nobody's place
+    const dim3 grid(Hk * sets, B, cut.nsplit);
     if (hd <= 64) launch((k_blk_step<E, 64>), grid, dim3(kBaThreads), 0, st, p);
     else launch((k_blk_step<E, 128>), grid, dim3(kBaThreads), 0, st, p);
-    if (cut.nsplit > 1) launch(k_blk_step_join<E>, dim3(H, B), dim3(kJoinThreads), 0, st, p);
+    if (cut.nsplit > 1) launch(k_blk_step_join<E>, dim3(H, B), dim3(kBaThreads), 0, st, p);
     return launched();
   });
 }
@@ -220,7 +247,7 @@ int t2r_attn_blk_prefill(const void* q, int dtype, int64_t q_ld, const int8_t* k
       if (hd <= 64) launch((k_blk_tile<E, 64, CFG64>), grid, dim3(64 * NW64), 0, st, p);
       else launch((k_blk_tile<E, 128, CFG128>), grid, dim3(64 * NW128), 0, st, p);
     }
-    if (cut.nsplit > 1) launch(k_blk_rows_join<E>, dim3(cut.tiles * Hk, cut.cols / 4), block, 0, st, p, cut.cols);
+    if (cut.nsplit > 1) launch(k_blk_rows_join<E>, dim3(cut.tiles * Hk, cut.cols / kBaWaves), block, 0, st, p, cut.cols);
     return launched();
   });
 }
