@@ -482,9 +482,9 @@ T2R_DEV float q_pieces(int hd, const float (*x)[16], v8h_t (*qf)[Pieces<E>::kN][
 }
 
 // The softmax of 32 keys' scores s for a lane's column: this lane's 16 keys are 16 (lane / 32) + r, `left` of them (below 16
-// only if EDGE) are seen. Raises m where needed (o and l with it) and leaves the probabilities' pieces.
-template <int NP, int DT, bool EDGE>
-T2R_DEV void soft32(v16f_t& s, float sk, float lw, float iw, int left, float& m, float& l, v16f_t* o, v8h_t (*pf)[2]) {
+// only if EDGE) are seen. First the maximum, raised where needed (o and l with it) ...
+template <int DT, bool EDGE>
+T2R_DEV void soft_max(v16f_t& s, float sk, int left, float& m, float& l, v16f_t* o) {
   if constexpr (EDGE) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = r < left ? s[r] : kNegInf;
@@ -502,16 +502,23 @@ T2R_DEV void soft32(v16f_t& s, float sk, float lw, float iw, int left, float& m,
 #pragma unroll
     for (int i = 0; i < DT; ++i) o[i] *= al;
   }
+}
+// ... then the probabilities: that of key r, times its V block's share, as fp16 pieces ...
+template <int NP>
+T2R_DEV float soft_weight(float s, float sk, float add, v8h_t (*pf)[2], int r) {
+  const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s, sk, add));
+  const _Float16 h = (_Float16)w;
+  pf[0][r >> 3][r & 7] = h;
+  if (NP == 2) pf[NP - 1][r >> 3][r & 7] = (_Float16)__builtin_fmaf((float)h, -1.0f, w);        // (one mixed-precision step)
+  return w;
+}
+// ... of all 16, and their sum into l.
+template <int NP>
+T2R_DEV void soft_exp(const v16f_t& s, float sk, float lw, float iw, float m, float& l, v8h_t (*pf)[2]) {
   const float add = lw + kLift - (m == kNegInf ? 0.0f : m);
   float ls[4] = {0, 0, 0, 0};
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sk, add));
-    ls[r & 3] += w;
-    const _Float16 h = (_Float16)w;
-    pf[0][r >> 3][r & 7] = h;
-    if (NP == 2) pf[NP - 1][r >> 3][r & 7] = (_Float16)__builtin_fmaf((float)h, -1.0f, w);      // (one mixed-precision step)
-  }
+  for (int r = 0; r < 16; ++r) ls[r & 3] += soft_weight<NP>(s[r], sk, add, pf, r);
   l = __builtin_fmaf((ls[0] + ls[1]) + (ls[2] + ls[3]), iw, l);
 }
 
@@ -696,8 +703,9 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_few(BlkAttn p) {
       if (more) load_k(st + kBaWaves);
       const int ch = st * 2 + c2;
       v8h_t pf[NP][2];
-      soft32<NP, DT, edge.value>(s, score_scale(sq, sg.ks[ch]), sg.lw[ch], sg.iw[ch],
-                                 edge.value ? keys_left(at, seg + ch * 16, sg.seen[ch]) : 16, m, l, o[0], pf);
+      const float sk = score_scale(sq, sg.ks[ch]);
+      soft_max<DT, edge.value>(s, sk, edge.value ? keys_left(at, seg + ch * 16, sg.seen[ch]) : 16, m, l, o[0]);
+      soft_exp<NP>(s, sk, sg.lw[ch], sg.iw[ch], m, l, pf);
 #pragma unroll
       for (int i = 0; i < DT; ++i)
 #pragma unroll
@@ -724,13 +732,17 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_few(BlkAttn p) {
 // LDS of k_blk_tile, in 16-byte slots: a fragment (64 lanes' operand of one MFMA) is 64 slots. K's fragments of a stage are
 // [kg][u][half], V's [kg][i][half]. The lane's slot is turned by the fragment's place, so that the loading threads, which
 // hold neighbouring 16-byte pieces of a token or channel, write to different banks.
-template <class E, int HD, int CT, int CG, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void k_blk_tile(BlkAttn p) {
-  constexpr int NP = Pieces<E>::kN, KU = HD / 32, DT = HD / 32, KG = NW / CG, COLS = 32 * CT * CG, THREADS = 64 * NW;
-  constexpr int STAGE = 32 * KG, FR = KG * KU * 2, PIECES = STAGE * HD / 16, PER = 2 * PIECES / THREADS;   // 16-byte pieces of K (as many of V)
-  using End = TileEnd<E, HD, CT, CG, NW>;
-  constexpr int kBufs = 2 * 2 * FR * 1024;
-  static_assert(PER * THREADS == 2 * PIECES && PIECES % 64 == 0, "whole loads");
+//
+// The waves of the two workgroups that share a SIMD drift apart, so that one's products run beside the other's softmax. What a
+// wave has to wait for is kept off its own path: a stage's codes are loaded a stage ahead, its V fragments are read from LDS
+// before the softmax, and two buffers leave one barrier a stage.
+template <class E, int HD, int CT, int CG>
+__global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
+  constexpr int NP = Pieces<E>::kN, KU = HD / 32, DT = HD / 32, KG = kBaWaves / CG, COLS = 32 * CT * CG;
+  constexpr int STAGE = 32 * KG, FR = KG * KU * 2, PIECES = STAGE * HD / 16, PER = PIECES / kBaThreads;   // 16-byte pieces of K, of V
+  using End = TileEnd<E, HD, CT, CG, kBaWaves>;
+  constexpr int kBufs = 4 * FR * 1024;
+  static_assert(PER * kBaThreads == PIECES, "whole loads");
   __shared__ BaSeg sg;
   __shared__ typename End::Ml ml;
   __shared__ __align__(16) char s_big[kBufs > End::kBytes ? kBufs : End::kBytes];
@@ -760,53 +772,51 @@ __global__ __launch_bounds__(64 * NW, 2) void k_blk_tile(BlkAttn p) {
   }
   const long long all_see = t.s.p0 + t.i0 + 1;                // keys below this are seen by every row
   const int tile = p.c.tile_bytes();
-  v4i_t raw[PER];
-  // Piece j: of K token j / (HD / 16), channels 16 (j % (HD / 16)); past K's, of V channel j / (2 KG), tokens 16 (j % (2 KG)).
-  // (Which of them a wave's i-th is does not depend on the lane.)
-  auto of_v = [&](int i) { return PIECES % THREADS == 0 ? i >= PIECES / THREADS : wave * 64 + i * THREADS >= PIECES; };
-  auto load = [&](int st) {
+  v4i_t kr[PER], vr[PER];
+  // piece j of K: token j / (HD / 16), channels 16 (j % (HD / 16)); of V: channel j / (2 KG), tokens 16 (j % (2 KG))
+  auto load_k = [&](int st) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int j = tid + i * THREADS;
-      if (!of_v(i)) {
-        const int key = st * STAGE + j / (HD / 16), d = j % (HD / 16) * 16;
-        raw[i] = *(const v4i_t*)(p.c.kc + (long long)sg.tb[key >> 4] * tile + ((key & bmask) * hd + (d < hd ? d : 0)));
-      } else {
-        const int jv = j - PIECES, ch = st * 2 * KG + jv % (2 * KG), d = jv / (2 * KG);
-        raw[i] = *(const v4i_t*)(p.c.vc + (long long)sg.tb[ch] * tile + (((ch * 16) & bmask) + (min(d, hd - 1) << lbs)));
-      }
+      const int j = tid + i * kBaThreads, key = st * STAGE + j / (HD / 16), d = j % (HD / 16) * 16;
+      kr[i] = *(const v4i_t*)(p.c.kc + (long long)sg.tb[key >> 4] * tile + ((key & bmask) * hd + (d < hd ? d : 0)));
     }
   };
-  auto put = [&](v8h_t* buf) {
+  auto load_v = [&](int st) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int j = tid + i * THREADS;
-      int fr, slot;
-      if (!of_v(i)) {
-        const int key = j / (HD / 16), dc = j % (HD / 16), k16 = key & 15;
-        fr = (key >> 5) * KU * 2 + (dc >> 1) * 2;
-        slot = ((dc & 1) * 32 + 8 * (k16 >> 2) + 4 * (key >> 4 & 1) + (k16 & 3)) ^ (dc & 7);    // (the token's row of the 32)
-      } else {
-        const int jv = j - PIECES, ck = jv % (2 * KG), d = jv / (2 * KG);
-        fr = FR + (ck >> 1) * DT * 2 + (d >> 5) * 2;
-        slot = ((ck & 1) * 32 + (d & 31)) ^ (2 * ck & 7);
-      }
-      buf[fr * 64 + slot] = codes_h(raw[i][0], raw[i][1]);
-      buf[(fr + 1) * 64 + slot] = codes_h(raw[i][2], raw[i][3]);
+      const int j = tid + i * kBaThreads, ch = st * 2 * KG + j % (2 * KG), d = j / (2 * KG);
+      vr[i] = *(const v4i_t*)(p.c.vc + (long long)sg.tb[ch] * tile + (((ch * 16) & bmask) + (min(d, hd - 1) << lbs)));
+    }
+  };
+  // half of a loaded piece (K's PER, then V's) into its fragment
+  auto put_half = [&](v8h_t* buf, int h) {
+    const int i = h >> 1, half = h & 1;
+    int fr, slot;
+    if (i < PER) {
+      const int j = tid + i * kBaThreads, key = j / (HD / 16), dc = j % (HD / 16), k16 = key & 15;
+      fr = (key >> 5) * KU * 2 + (dc >> 1) * 2;
+      slot = ((dc & 1) * 32 + 8 * (k16 >> 2) + 4 * (key >> 4 & 1) + (k16 & 3)) ^ (dc & 7);   // (the token's row of the 32)
+      buf[(fr + half) * 64 + slot] = codes_h(kr[i][2 * half], kr[i][2 * half + 1]);
+    } else {
+      const int j = tid + (i - PER) * kBaThreads, ck = j % (2 * KG), d = j / (2 * KG);
+      fr = FR + (ck >> 1) * DT * 2 + (d >> 5) * 2;
+      slot = ((ck & 1) * 32 + (d & 31)) ^ (2 * ck & 7);
+      buf[(fr + half) * 64 + slot] = codes_h(vr[i - PER][2 * half], vr[i - PER][2 * half + 1]);
     }
   };
   // a segment's blocks, and its first loads
   auto begin = [&](int n) {
     seg_blocks(sg, p.c, blk, kvh, n, STAGE);
-    load(0);
+    load_k(0);
+    load_v(0);
   };
   begin((int)min((long long)kBaSeg, kend - k0));
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) sq[ct] = p.a * q_pieces<E, KU>(hd, x[ct], qf[ct]);
   for (long long seg = k0; seg < kend; seg += kBaSeg) {
-    const int n = (int)min((long long)kBaSeg, kend - seg), stages = (n + STAGE - 1) / STAGE;
+    const int n = (int)min((long long)kBaSeg, kend - seg), stages = (n + STAGE - 1) / STAGE, last = stages - 1;
     bool holes;
-    const float vmax = seg_scales<NW>(sg, p.c, blk, kvh, n, STAGE, vref, &holes);
+    const float vmax = seg_scales<kBaWaves>(sg, p.c, blk, kvh, n, STAGE, vref, &holes);
     if (vmax > vref) {
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct)
@@ -814,49 +824,91 @@ __global__ __launch_bounds__(64 * NW, 2) void k_blk_tile(BlkAttn p) {
         for (int i = 0; i < DT; ++i) o[ct][i] *= vref / vmax;
     }
     vref = vmax;
-    auto stage = [&](int st, auto edge) {
-      v8h_t* buf = bufs + (st & 1) * 2 * FR * 64;
-      put(buf);
-      __syncthreads();                                        // (the stage before last, in this buffer, is read: all were past it here)
-      if (st + 1 < stages) load(st + 1);
-      const int key0 = st * STAGE + kg * 32, ch = (key0 >> 4) + c2;
-      if (key0 >= n) return;
-      v16f_t s[CT];
+    // (past the last stage loads repeat it, and nobody reads what is put of them)
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) s[ct] = v16f_t{};
+    for (int h = 0; h < 4 * PER; ++h) put_half(bufs, h);
+    load_k(min(1, last));
+    load_v(min(1, last));
+    __syncthreads();
+    auto stage = [&](int st, auto edge) {
+      const v8h_t* buf = bufs + (st & 1) * 2 * FR * 64;
+      const int ch = ((st * STAGE + kg * 32) >> 4) + c2;
+      v8h_t kf[KU][2], vf[DT][2];
 #pragma unroll
       for (int u = 0; u < KU; ++u)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const v8h_t kf = buf[((kg * KU + u) * 2 + half) * 64 + (lane ^ ((2 * u + c2) & 7))];
-#pragma unroll
-          for (int q = 0; q < NP; ++q)
-#pragma unroll
-            for (int ct = 0; ct < CT; ++ct) s[ct] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[ct][u][q][half], s[ct], 0, 0, 0);
-        }
+        for (int half = 0; half < 2; ++half) kf[u][half] = buf[((kg * KU + u) * 2 + half) * 64 + (lane ^ ((2 * u + c2) & 7))];
       const float ks = sg.ks[ch], lw = sg.lw[ch], iw = sg.iw[ch];
       const int seen = edge.value ? sg.seen[ch] : 16;
-      v8h_t pf[CT][NP][2];
+      __builtin_amdgcn_sched_barrier(0);
+      // The scores; between their products, which follow from one another, the next stage's codes are converted. (The order is
+      // pinned: left to itself the compiler puts all of one before all of the other.)
+      v16f_t s[CT];
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
-        soft32<NP, DT, edge.value>(s[ct], score_scale(sq[ct], ks), lw, iw, edge.value ? keys_left(at[ct], seg + ch * 16, seen) : 16,
-                                   m[ct], l[ct], o[ct], pf[ct]);
+      for (int ct = 0; ct < CT; ++ct) s[ct] = v16f_t{};
+      v8h_t* next = bufs + (~st & 1) * 2 * FR * 64;
+      constexpr int GROUPS = KU * 2, EACH = 4 * PER / GROUPS;
+      static_assert(EACH * GROUPS == 4 * PER, "the same number of pieces a group");
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {
+#pragma unroll
+        for (int q = 0; q < NP; ++q)
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct)
+            s[ct] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[g >> 1][g & 1], qf[ct][g >> 1][q][g & 1], s[ct], 0, 0, 0);
+#pragma unroll
+        for (int h = 0; h < EACH; ++h) put_half(next, g * EACH + h);
+        __builtin_amdgcn_sched_barrier(0);
+      }
 #pragma unroll
       for (int i = 0; i < DT; ++i)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const v8h_t vf = buf[(FR + (kg * DT + i) * 2 + half) * 64 + (lane ^ (2 * (2 * kg + c2) & 7))];
+        for (int half = 0; half < 2; ++half)
+          vf[i][half] = buf[(FR + (kg * DT + i) * 2 + half) * 64 + (lane ^ (2 * (2 * kg + c2) & 7))];
+      __builtin_amdgcn_sched_barrier(0);
+      v8h_t pf[CT][NP][2];
+      float sk[CT], add[CT], ls[CT][2];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        sk[ct] = score_scale(sq[ct], ks);
+        soft_max<DT, edge.value>(s[ct], sk[ct], edge.value ? keys_left(at[ct], seg + ch * 16, seen) : 16, m[ct], l[ct], o[ct]);
+        add[ct] = lw + kLift - (m[ct] == kNegInf ? 0.0f : m[ct]);
+        ls[ct][0] = ls[ct][1] = 0;
+      }
+      // The probabilities of 8 keys, then their products; the other 8 keys' between those, the next loads between the last.
+      auto weigh = [&](int r) {
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) ls[ct][r & 1] += soft_weight<NP>(s[ct][r], sk[ct], add[ct], pf[ct], r);
+      };
+#pragma unroll
+      for (int r = 0; r < 8; ++r) weigh(r);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int i = 0; i < DT; ++i) {
 #pragma unroll
           for (int q = 0; q < NP; ++q)
 #pragma unroll
-            for (int ct = 0; ct < CT; ++ct) o[ct][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[ct][q][half], o[ct][i], 0, 0, 0);
+            for (int ct = 0; ct < CT; ++ct) o[ct][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[i][half], pf[ct][q][half], o[ct][i], 0, 0, 0);
+          if (half == 0) {
+#pragma unroll
+            for (int r = 0; r < 8 / DT; ++r) weigh(8 + i * (8 / DT) + r);
+          } else if (i == 0) {
+            load_k(min(st + 2, last));
+          } else if (i == 1) {
+            load_v(min(st + 2, last));
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) l[ct] = __builtin_fmaf(ls[ct][0] + ls[ct][1], iw, l[ct]);
+      __syncthreads();                                        // this buffer is read, the other one whole
     };
     const int plain = plain_steps(all_see, seg, n, STAGE, holes);
     int st = 0;
     for (; st < plain; ++st) stage(st, std::false_type());
     for (; st < stages; ++st) stage(st, std::true_type());
-    __syncthreads();                                          // the next segment's tables and stages, or the sums, take their place
     const long long next = seg + kBaSeg;
     if (next < kend) {
       const int m2 = (int)min((long long)kBaSeg, kend - next);
@@ -864,7 +916,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_blk_tile(BlkAttn p) {
       begin(m2);
     }
   }
-  tile_end<E, HD, CT, CG, NW>(p, t, kvh, blockIdx.y, k0 == 0 && kend == t.end, vref, m, l, o, ml, (float*)s_big);
+  tile_end<E, HD, CT, CG, kBaWaves>(p, t, kvh, blockIdx.y, k0 == 0 && kend == t.end, vref, m, l, o, ml, (float*)s_big);
 }
 
 // Joins the parts of a tile's columns: a wave a column

@@ -238,14 +238,8 @@ int t2r_attn_blk_prefill(const void* q, int dtype, int64_t q_ld, const int8_t* k
       if (hd <= 64) launch((k_blk_few<E, 64>), grid, block, 0, st, p);
       else launch((k_blk_few<E, 128>), grid, block, 0, st, p);
     } else {
-#ifndef CFG64
-#define CFG64 CT, 2, 4
-#define CFG128 1, 2, 4
-#define NW64 4
-#define NW128 4
-#endif
-      if (hd <= 64) launch((k_blk_tile<E, 64, CFG64>), grid, dim3(64 * NW64), 0, st, p);
-      else launch((k_blk_tile<E, 128, CFG128>), grid, dim3(64 * NW128), 0, st, p);
+      if (hd <= 64) launch((k_blk_tile<E, 64, CT, 2>), grid, block, 0, st, p);
+      else launch((k_blk_tile<E, 128, 1, 2>), grid, block, 0, st, p);
     }
     if (cut.nsplit > 1) launch(k_blk_rows_join<E>, dim3(cut.tiles * Hk, cut.cols / kBaWaves), block, 0, st, p, cut.cols);
     return launched();
