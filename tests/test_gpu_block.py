@@ -365,6 +365,28 @@ def test_rows_over_several_segments(env, Hk, hd, dtype):
     check(torch, got, want, bound, dtype)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("H,Hk,hd,block,news,lens", [
+    (32, 8, 64, 64, [2100], [2100]),
+    (30, 3, 48, 32, [1203, 1, 0, 1500], [1300, 70, 10, 3000]),               # (10 heads a group: 12 rows a tile of 128 columns)
+    (96, 3, 16, 16, [33, 700], [33, 2500]),
+])
+def test_many_rows(env, H, Hk, hd, block, news, lens, dtype):
+    """Prompts long enough for the widest tiles at small head dims. A few rows are compared, each tile's end among them."""
+    torch, ops = env
+    rng = np.random.default_rng(18)
+    c = Both(torch, ops, rng, lens, Hk, hd, block).fill(rng, spread=1.5).send()
+    starts = np.concatenate([[0], np.cumsum(news)])
+    rows = int(starts[-1])
+    assert rows * H > 64 * 1024
+    x, t = rounded(torch, rng.standard_normal((rows, H * hd)), dtype)
+    got = ops.attention_block_prefill(t, *c.dev, i32(torch, starts), c.lens_d, H)
+    rt = 128 * Hk // H
+    only = sorted({r for r in (0, rt - 1, rt, 2 * rt - 1, 32, 700, news[0] - 1, news[0], rows // 2, rows - rt - 1, rows - 2, rows - 1)})
+    want, bound = attention(c.host, x, c.table, starts, lens, H, 1 / math.sqrt(hd), 0 if dtype == "f32" else 2.0 ** -11, only=only)
+    check(torch, got, want, bound, dtype)
+
+
 def test_many_sequences_with_few_rows(env):
     """More sequences than a wave has lanes, most of them without rows."""
     torch, ops = env

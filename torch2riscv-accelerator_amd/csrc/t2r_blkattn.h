@@ -509,7 +509,9 @@ T2R_DEV float soft_weight(float s, float sk, float add, v8h_t (*pf)[2], int r) {
   const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s, sk, add));
   const _Float16 h = (_Float16)w;
   pf[0][r >> 3][r & 7] = h;
-  if (NP == 2) pf[NP - 1][r >> 3][r & 7] = (_Float16)__builtin_fmaf((float)h, -1.0f, w);        // (one mixed-precision step)
+  float minus = -1.0f;                                        // (kept from the compiler, which would take h out of fp16 to subtract it:
+  asm("" : "+s"(minus));                                      // so it is one mixed-precision step)
+  if (NP == 2) pf[NP - 1][r >> 3][r & 7] = (_Float16)__builtin_fmaf((float)h, minus, w);
   return w;
 }
 // ... of all 16, and their sum into l.
@@ -834,16 +836,19 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
       const v8h_t* buf = bufs + (st & 1) * 2 * FR * 64;
       const int ch = ((st * STAGE + kg * 32) >> 4) + c2;
       v8h_t kf[KU][2], vf[DT][2];
+      auto read_k = [&](int from, int to) {
 #pragma unroll
-      for (int u = 0; u < KU; ++u)
+        for (int u = from; u < to; ++u)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) kf[u][half] = buf[((kg * KU + u) * 2 + half) * 64 + (lane ^ ((2 * u + c2) & 7))];
+          for (int half = 0; half < 2; ++half) kf[u][half] = buf[((kg * KU + u) * 2 + half) * 64 + (lane ^ ((2 * u + c2) & 7))];
+      };
+      read_k(0, KU / 2);                                      // (the others follow while these are used)
       const float ks = sg.ks[ch], lw = sg.lw[ch], iw = sg.iw[ch];
       const int seen = edge.value ? sg.seen[ch] : 16;
       __builtin_amdgcn_sched_barrier(0);
-      // The scores; between their products, which follow from one another, the next stage's codes are converted. (The order is
-      // pinned: left to itself the compiler puts all of one before all of the other.)
-      v16f_t s[CT];
+      // The scores; between their products the next stage's codes are converted. (The order is pinned: left to itself the
+      // compiler puts all of one before all of the other.)
+            v16f_t s[CT];
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) s[ct] = v16f_t{};
       v8h_t* next = bufs + (~st & 1) * 2 * FR * 64;
@@ -854,17 +859,17 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
 #pragma unroll
         for (int q = 0; q < NP; ++q)
 #pragma unroll
-          for (int ct = 0; ct < CT; ++ct)
-            s[ct] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[g >> 1][g & 1], qf[ct][g >> 1][q][g & 1], s[ct], 0, 0, 0);
+          for (int ct = 0; ct < CT; ++ct) s[ct] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[g >> 1][g & 1], qf[ct][g >> 1][q][g & 1], s[ct], 0, 0, 0);
+        if (g == 0) read_k(KU / 2, KU);
 #pragma unroll
         for (int h = 0; h < EACH; ++h) put_half(next, g * EACH + h);
         __builtin_amdgcn_sched_barrier(0);
       }
+      auto read_v = [&](int half) {
 #pragma unroll
-      for (int i = 0; i < DT; ++i)
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-          vf[i][half] = buf[(FR + (kg * DT + i) * 2 + half) * 64 + (lane ^ (2 * (2 * kg + c2) & 7))];
+        for (int i = 0; i < DT; ++i) vf[i][half] = buf[(FR + (kg * DT + i) * 2 + half) * 64 + (lane ^ (2 * (2 * kg + c2) & 7))];
+      };
+      read_v(0);
       __builtin_amdgcn_sched_barrier(0);
       v8h_t pf[CT][NP][2];
       float sk[CT], add[CT], ls[CT][2];
@@ -886,17 +891,17 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
 #pragma unroll
       for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int i = 0; i < DT; ++i) {
+        for (int g = 0; g < NP * DT; ++g) {
+          const int q = g / DT, i = g % DT;
 #pragma unroll
-          for (int q = 0; q < NP; ++q)
-#pragma unroll
-            for (int ct = 0; ct < CT; ++ct) o[ct][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[i][half], pf[ct][q][half], o[ct][i], 0, 0, 0);
+          for (int ct = 0; ct < CT; ++ct) o[ct][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[i][half], pf[ct][q][half], o[ct][i], 0, 0, 0);
           if (half == 0) {
+            if (g == 0) read_v(1);
 #pragma unroll
-            for (int r = 0; r < 8 / DT; ++r) weigh(8 + i * (8 / DT) + r);
-          } else if (i == 0) {
+            for (int r = 8 + g * 8 / (NP * DT); r < 8 + (g + 1) * 8 / (NP * DT); ++r) weigh(r);
+          } else if (g == 0) {
             load_k(min(st + 2, last));
-          } else if (i == 1) {
+          } else if (g == 1) {
             load_v(min(st + 2, last));
           }
           __builtin_amdgcn_sched_barrier(0);

@@ -12,10 +12,6 @@
 
 using namespace t2r;
 
-#ifndef COLS64
-#define COLS64 (dtype != T2R_F32 ? 128 : 64)
-#define COLS128 64
-#endif
 namespace {
 
 inline int launched() { return hipGetLastError() == hipSuccess ? T2R_OK : T2R_EHIP; }
@@ -80,12 +76,15 @@ Cut step_cut(int B, int H, int Hk, int hd, int block, int width, int dtype) {
   c.nsplit = (int)cdiv(cap, c.chunk);
   return c;
 }
-Cut rows_cut(int B, int rows, int H, int Hk, int hd, int block, int width, int dtype) {
+Cut rows_cut(int B, int rows, int H, int Hk, int hd, int block, int width) {
   const long long cap = (long long)width * block;
   const int G = H / Hk;
   Cut c;
-  // few rows: one tile of 32 columns a sequence; else 64, or 128 where a wave's registers hold two times 32 columns
-  c.cols = (long long)rows * G <= 32LL * B ? 32 : hd <= 64 ? COLS64 : COLS128;
+  // Few rows: one tile of 32 columns a sequence. Else 64; 128, which a conversion of codes then serves, at head dims whose sums
+  // leave a wave registers for two times 32, once 64 would be more than the chip has places for twice (1024). 32 heads of 64,
+  // one prompt of 512 / 2032 / 4064 rows, us: fp32 13.6 / 55.2 / 186 in 64 columns and 18.8 / 56.0 / 174 in 128, bf16 11.6 /
+  // 40.8 / 130 and 15.0 / 40.2 / 116.
+  c.cols = (long long)rows * G <= 32LL * B ? 32 : hd <= 64 && (long long)rows * H > 64 * 1024 ? 128 : 64;
   const int rt = c.cols / G;
   // every sequence's last tile may be a part of one
   const long long tiles = rows / rt + (B < rows ? B : rows);
@@ -172,7 +171,7 @@ int t2r_kv_read_blk(const int8_t* kc, const int8_t* vc, const float* ks, const f
 
 int64_t t2r_attn_blk_workspace_bytes(int B, int rows, int H, int Hk, int hd, int block, int width, int dtype) {
   if (B <= 0 || rows < 0 || !attn_shape_ok(H, Hk) || hd <= 0 || block <= 0 || width <= 0 || !dtype_ok(dtype)) return -1;
-  return rows == 0 ? step_ws(step_cut(B, H, Hk, hd, block, width, dtype), B, H, hd) : rows_ws(rows_cut(B, rows, H, Hk, hd, block, width, dtype), Hk, hd);
+  return rows == 0 ? step_ws(step_cut(B, H, Hk, hd, block, width, dtype), B, H, hd) : rows_ws(rows_cut(B, rows, H, Hk, hd, block, width), Hk, hd);
 }
 
 int t2r_attn_blk_decode(const void* q, int dtype, int64_t q_ld, const int8_t* kc, const int8_t* vc, const float* ks,
@@ -218,7 +217,7 @@ int t2r_attn_blk_prefill(const void* q, int dtype, int64_t q_ld, const int8_t* k
   std::memset(&p, 0, sizeof(p));
   if (int rc = cache_args(kc, vc, ks, vs, n_blocks, block, Hk, hd, table, width, &p.c)) return rc;
   if (!attn_shape_ok(H, Hk) || B <= 0 || rows <= 0 || q_ld < (int64_t)H * hd || out_ld < (int64_t)H * hd) return T2R_ESHAPE;
-  const Cut cut = rows_cut(B, rows, H, Hk, hd, block, width, dtype);
+  const Cut cut = rows_cut(B, rows, H, Hk, hd, block, width);
   if (cut.nsplit > 65535 || (long long)cut.tiles * Hk > INT32_MAX) return T2R_ESHAPE;
   const long long need = rows_ws(cut, Hk, hd);
   if (need > 0 && (!workspace || workspace_bytes < need || misaligned(workspace, 16))) return T2R_ENOMEM;
@@ -233,13 +232,14 @@ int t2r_attn_blk_prefill(const void* q, int dtype, int64_t q_ld, const int8_t* k
   return by_type(dtype, [&](auto e) {
     using E = decltype(e);
     const dim3 grid(cut.tiles * Hk, cut.nsplit), block(kBaThreads);
-    constexpr int CT = sizeof(E) == 2 ? 2 : 1;
     if (cut.cols == 32) {
       if (hd <= 64) launch((k_blk_few<E, 64>), grid, block, 0, st, p);
       else launch((k_blk_few<E, 128>), grid, block, 0, st, p);
-    } else {
-      if (hd <= 64) launch((k_blk_tile<E, 64, CT, 2>), grid, block, 0, st, p);
+    } else if (cut.cols == 64) {
+      if (hd <= 64) launch((k_blk_tile<E, 64, 1, 2>), grid, block, 0, st, p);
       else launch((k_blk_tile<E, 128, 1, 2>), grid, block, 0, st, p);
+    } else {
+      launch((k_blk_tile<E, 64, 2, 2>), grid, block, 0, st, p);
     }
     if (cut.nsplit > 1) launch(k_blk_rows_join<E>, dim3(cut.tiles * Hk, cut.cols / kBaWaves), block, 0, st, p, cut.cols);
     return launched();
