@@ -173,7 +173,7 @@ enum { T2R_F32 = 0, T2R_BF16 = 1, T2R_F16 = 2 };
  * table, holds no tokens: appended rows are dropped there, the attention leaves its positions out, reads give zeros.
  * A block that is appended to belongs to one sequence (full blocks may be shared by tables).
  * Ragged rows: those of sequence b are starts[b] .. starts[b + 1] - 1 (starts [B + 1], device, not decreasing) and the
- * last of them stands at position lens[b] - 1 (device); rows outside every sequence are left alone.
+ * last of them stands at position lens[b] - 1 (device); rows outside every sequence are left alone. rows < 2^24.
  *
  * Appends rows k, v [rows, Hk * hd], k_ld / v_ld elements apart (columns of a q | k | v matrix, say). In each block and
  * head that rows enter: s = F(max |x| / 127) over its new rows, or its present scale where that is larger and the block
@@ -189,8 +189,10 @@ int t2r_kv_read_blk(const int8_t* kc, const int8_t* vc, const float* ks, const f
                     int dtype, void* k, void* v, void* stream);
 /* Attention over that cache, out = softmax(scale q K^T) V, H / Hk <= 32 query heads a KV head; q [.., H * hd] and out of
  * the same type, q_ld / out_ld elements from row to row (out may be q). scale > 0. A row that sees no position (an idle
- * sequence, or one whose table has no blocks there) gives zeros.
- * _decode: row b is sequence b's newest token and sees positions 0 .. lens[b] - 1; B <= 65535.
+ * sequence, or one whose table has no blocks there) gives zeros, one with a NaN in it NaN; what one with an infinity, or
+ * with scores past fp32's range, gives is not defined.
+ * _decode: row b is sequence b's newest token and sees positions 0 .. lens[b] - 1; B <= 65535, and a table
+ * spans less than 2^27 positions.
  * _prefill: ragged rows, each sees the positions up to its own. A row below position 0 (lens[b] less than the sequence's
  * rows) has no place in its sequence and gives NaN.
  * Workspace (device, 16-byte aligned): t2r_attn_blk_workspace_bytes with rows = 0 for _decode; 0 bytes may be NULL. It is

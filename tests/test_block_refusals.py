@@ -37,7 +37,8 @@ BAD_CACHE = [(dict(kc=None), abi.T2R_EINVAL), (dict(vs=None), abi.T2R_EINVAL), (
              (dict(n=1 << 30, Hk=4), abi.T2R_ESHAPE), (dict(width=1 << 26), abi.T2R_ESHAPE), (dict(B=0), abi.T2R_ESHAPE)]
 
 
-@pytest.mark.parametrize("kw,code", BAD_CACHE + [(dict(rows=0), abi.T2R_ESHAPE), (dict(k_ld=127), abi.T2R_ESHAPE), (dict(v=ODD), abi.T2R_EINVAL),
+@pytest.mark.parametrize("kw,code", BAD_CACHE + [(dict(rows=0), abi.T2R_ESHAPE), (dict(rows=1 << 24), abi.T2R_ESHAPE),
+                                                 (dict(k_ld=127), abi.T2R_ESHAPE), (dict(v_ld=64), abi.T2R_ESHAPE), (dict(v=ODD), abi.T2R_EINVAL),
                                                  (dict(starts=None), abi.T2R_EINVAL)])
 def test_append_refuses(kw, code):
     assert append(abi.load(), **kw) == code
@@ -58,7 +59,10 @@ def test_attention_refuses(form, kw, code):
 def test_attention_refuses_its_own():
     lib = abi.load()
     assert attend(lib, "decode", B=65536) == abi.T2R_ESHAPE
-    assert attend(lib, "prefill", rows=0) == abi.T2R_ESHAPE
+    assert attend(lib, "decode", width=1 << 20) == abi.T2R_ENOMEM and attend(lib, "decode", width=1 << 22) == abi.T2R_ESHAPE
+    assert attend(lib, "prefill", rows=0) == abi.T2R_ESHAPE and attend(lib, "prefill", rows=1 << 24) == abi.T2R_ESHAPE
+    # (more workgroups than a launch has threads for: 2^23 rows in tiles of one row and 4 KV heads)
+    assert attend(lib, "prefill", rows=1 << 23, H=128, Hk=4, hd=128, q_ld=1 << 14, out_ld=1 << 14, width=64) == abi.T2R_ESHAPE
     assert attend(lib, "prefill", starts=None) == abi.T2R_EINVAL
     assert lib.t2r_attn_blk_workspace_bytes(1, 0, 4, 2, 64, 64, 2, 0) == 0
     assert lib.t2r_attn_blk_workspace_bytes(1, 0, 4, 2, 64, 64, 128, 0) > 0
@@ -69,7 +73,7 @@ def test_attention_refuses_its_own():
 def test_read_refuses():
     lib = abi.load()
     ok = dict(kc=P, vc=P, ks=P, vs=P, n=4, block=64, Hk=2, hd=64, table=P, width=2, starts=P, lens=P, B=1, rows=1, dtype=0, k=P, v=P)
-    for kw, code in BAD_CACHE + [(dict(rows=0), abi.T2R_ESHAPE), (dict(k=None), abi.T2R_EINVAL)]:
+    for kw, code in BAD_CACHE + [(dict(rows=0), abi.T2R_ESHAPE), (dict(rows=1 << 24), abi.T2R_ESHAPE), (dict(k=None), abi.T2R_EINVAL)]:
         assert lib.t2r_kv_read_blk(*{**ok, **kw}.values(), None) == code
 
 
@@ -78,7 +82,7 @@ def test_logprobs_refuses():
     ok = dict(x=P, dtype=0, ld=100, tokens=P, rows=2, V=100, top=3, lp=P, ent=P, ids=P, val=P, ws=P, ws_bytes=1 << 20)
     for kw, code in ((dict(x=None), abi.T2R_EINVAL), (dict(tokens=None), abi.T2R_EINVAL), (dict(ids=None), abi.T2R_EINVAL),
                      (dict(val=None), abi.T2R_EINVAL), (dict(dtype=-1), abi.T2R_EINVAL), (dict(x=ODD), abi.T2R_EINVAL),
-                     (dict(rows=0), abi.T2R_ESHAPE), (dict(V=0), abi.T2R_ESHAPE), (dict(ld=99), abi.T2R_ESHAPE),
+                     (dict(rows=0), abi.T2R_ESHAPE), (dict(rows=1 << 24), abi.T2R_ESHAPE), (dict(V=0), abi.T2R_ESHAPE), (dict(ld=99), abi.T2R_ESHAPE),
                      (dict(top=-1), abi.T2R_ERANGE), (dict(top=33), abi.T2R_ERANGE), (dict(V=2, top=3), abi.T2R_ERANGE),
                      (dict(V=20000, ld=20000, ws=None), abi.T2R_ENOMEM), (dict(V=20000, ld=20000, ws_bytes=10), abi.T2R_ENOMEM)):
         assert lib.t2r_logprobs(*{**ok, **kw}.values(), None) == code, kw

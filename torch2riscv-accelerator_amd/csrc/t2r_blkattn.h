@@ -89,8 +89,8 @@ struct BaSeg {
   int tb[kBaSeg / 16];                        // (0 where there is none)
   int seen[kBaSeg / 16];                      // 16, or fewer at the end, or none
   float ks[kBaSeg / 16], lw[kBaSeg / 16], iw[kBaSeg / 16];
-  float red[8];
-  int holes[8];
+  float red[kBaWaves];
+  int holes[kBaWaves];
 };
 // The tables of the keys key0 .. key0 + n - 1, in whole steps of `step` keys, for the whole workgroup. In parts, so that what
 // a kernel has to load meanwhile is asked for between them: seg_table asks for this thread's table entry; seg_blocks puts the
@@ -108,7 +108,6 @@ T2R_DEV void seg_blocks(BaSeg& sg, const BlkCache& c, int blk, int head, int n, 
   }
   __syncthreads();
 }
-template <int NW>
 T2R_DEV float seg_scales(BaSeg& sg, const BlkCache& c, int blk, int head, int n, int step, float vref, bool* holes) {
   const int tid = threadIdx.x, wave = wave_index(), entries = (n + step - 1) / step * (step >> 4);
   float ks = 0, vs = 0;
@@ -127,7 +126,7 @@ T2R_DEV float seg_scales(BaSeg& sg, const BlkCache& c, int blk, int head, int n,
   float m = vref;
   int any = 0;
 #pragma unroll
-  for (int w = 0; w < NW; ++w) {
+  for (int w = 0; w < kBaWaves; ++w) {
     m = fmaxf(m, sg.red[w]);
     any |= sg.holes[w];
   }
@@ -207,7 +206,7 @@ __global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_step(BlkAt
     load_v(st);
   }
   bool holes;
-  const float vref = seg_scales<kBaWaves>(sg, p.c, mine, kvh, n, 64, 0.0f, &holes);
+  const float vref = seg_scales(sg, p.c, mine, kvh, n, 64, 0.0f, &holes);
   // q's pieces in the layout of K's rows, after the row's largest magnitude
   v8h_t qf[KU][2];
   float sq;
@@ -527,8 +526,8 @@ T2R_DEV void soft_exp(const v16f_t& s, float sk, float lw, float iw, float m, fl
 // The end of a tile: its waves' sums (wave's column group cg of 32 CT, key group kg of KG) are joined through LDS (so: KG x COLS
 // rows of HD + 4 floats, which keeps 16-byte accesses free of bank conflicts) and written as the result or, of a part of the
 // keys, into the workspace.
-template <class E, int HD, int CT, int CG, int NW> struct TileEnd {
-  static constexpr int KG = NW / CG, COLS = 32 * CT * CG, LD = HD + 4, kBytes = KG * COLS * LD * 4;
+template <int HD, int CT, int CG> struct TileEnd {
+  static constexpr int KG = kBaWaves / CG, COLS = 32 * CT * CG, LD = HD + 4, kBytes = KG * COLS * LD * 4;
   struct Ml { float m[KG][COLS], l[KG][COLS], top[COLS], sum[COLS], inv[COLS]; };
 };
 // four values side by side, at any element's alignment
@@ -536,10 +535,10 @@ template <class E> T2R_DEV void store4(E* p, v4f_t x) {
   struct __attribute__((packed, aligned(sizeof(E)))) V { E e[4]; };
   *(V*)p = V{{narrow<E>(x[0]), narrow<E>(x[1]), narrow<E>(x[2]), narrow<E>(x[3])}};
 }
-template <class E, int HD, int CT, int CG, int NW>
+template <class E, int HD, int CT, int CG>
 T2R_DEV void tile_end(const BlkAttn& p, const Tile& t, int kvh, int split, bool whole, float vref, float* m, float* l,
-                      v16f_t (*o)[HD / 32], typename TileEnd<E, HD, CT, CG, NW>::Ml& ml, float* so) {
-  using T = TileEnd<E, HD, CT, CG, NW>;
+                      v16f_t (*o)[HD / 32], typename TileEnd<HD, CT, CG>::Ml& ml, float* so) {
+  using T = TileEnd<HD, CT, CG>;
   constexpr int KG = T::KG, COLS = T::COLS, LD = T::LD, DT = HD / 32;
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_index(), col = lane & 31, c2 = lane >> 5;
   const int cg = wave % CG, kg = wave / CG, hd = p.c.hd, G = p.G, ncol = t.rows * G;
@@ -584,7 +583,7 @@ T2R_DEV void tile_end(const BlkAttn& p, const Tile& t, int kvh, int split, bool 
   const int d = tid % PER * 4;
   if (d >= hd) return;
 #pragma unroll 2
-  for (int cc = tid / PER; cc < ncol; cc += 64 * NW / PER) {
+  for (int cc = tid / PER; cc < ncol; cc += kBaThreads / PER) {
     v4f_t x = *(const v4f_t*)(so + cc * LD + d);
 #pragma unroll
     for (int w = 1; w < KG; ++w) x += *(const v4f_t*)(so + (w * COLS + cc) * LD + d);
@@ -633,7 +632,7 @@ template <class E, int HD>
 __global__ __launch_bounds__(kBaThreads, 2) void k_blk_few(BlkAttn p) {
   constexpr int NP = Pieces<E>::kN, KU = HD / 32, DT = HD / 32;
   __shared__ BaSeg sg;
-  using End = TileEnd<E, HD, 1, 1, kBaWaves>;
+  using End = TileEnd<HD, 1, 1>;
   __shared__ typename End::Ml ml;
   __shared__ __align__(16) char s_o[End::kBytes];
   const int lane = threadIdx.x & 63, wave = wave_index(), col = lane & 31, c2 = lane >> 5;
@@ -684,7 +683,7 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_few(BlkAttn p) {
   for (long long seg = k0; seg < kend; seg += kBaSeg) {
     const int n = (int)min((long long)kBaSeg, kend - seg), steps = (n + 31) >> 5;
     bool holes;
-    const float vmax = seg_scales<kBaWaves>(sg, p.c, blk, kvh, n, 32, vref, &holes);
+    const float vmax = seg_scales(sg, p.c, blk, kvh, n, 32, vref, &holes);
     if (vmax > vref) {
 #pragma unroll
       for (int i = 0; i < DT; ++i) o[0][i] *= vref / vmax;
@@ -728,7 +727,7 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_few(BlkAttn p) {
       begin(m);
     }
   }
-  tile_end<E, HD, 1, 1, kBaWaves>(p, t, kvh, blockIdx.y, k0 == 0 && kend == t.end, vref, &m, &l, o, ml, (float*)s_o);
+  tile_end<E, HD, 1, 1>(p, t, kvh, blockIdx.y, k0 == 0 && kend == t.end, vref, &m, &l, o, ml, (float*)s_o);
 }
 
 // LDS of k_blk_tile, in 16-byte slots: a fragment (64 lanes' operand of one MFMA) is 64 slots. K's fragments of a stage are
@@ -738,11 +737,11 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_few(BlkAttn p) {
 // The waves of the two workgroups that share a SIMD drift apart, so that one's products run beside the other's softmax. What a
 // wave has to wait for is kept off its own path: a stage's codes are loaded a stage ahead, its V fragments are read from LDS
 // before the softmax, and two buffers leave one barrier a stage.
-template <class E, int HD, int CT, int CG>
+template <class E, int HD, int CT>
 __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
-  constexpr int NP = Pieces<E>::kN, KU = HD / 32, DT = HD / 32, KG = kBaWaves / CG, COLS = 32 * CT * CG;
+  constexpr int NP = Pieces<E>::kN, KU = HD / 32, DT = HD / 32, CG = 2, KG = kBaWaves / CG, COLS = 32 * CT * CG;
   constexpr int STAGE = 32 * KG, FR = KG * KU * 2, PIECES = STAGE * HD / 16, PER = PIECES / kBaThreads;   // 16-byte pieces of K, of V
-  using End = TileEnd<E, HD, CT, CG, kBaWaves>;
+  using End = TileEnd<HD, CT, CG>;
   constexpr int kBufs = 4 * FR * 1024;
   static_assert(PER * kBaThreads == PIECES, "whole loads");
   __shared__ BaSeg sg;
@@ -818,7 +817,7 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
   for (long long seg = k0; seg < kend; seg += kBaSeg) {
     const int n = (int)min((long long)kBaSeg, kend - seg), stages = (n + STAGE - 1) / STAGE, last = stages - 1;
     bool holes;
-    const float vmax = seg_scales<kBaWaves>(sg, p.c, blk, kvh, n, STAGE, vref, &holes);
+    const float vmax = seg_scales(sg, p.c, blk, kvh, n, STAGE, vref, &holes);
     if (vmax > vref) {
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct)
@@ -921,7 +920,7 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
       begin(m2);
     }
   }
-  tile_end<E, HD, CT, CG, kBaWaves>(p, t, kvh, blockIdx.y, k0 == 0 && kend == t.end, vref, m, l, o, ml, (float*)s_big);
+  tile_end<E, HD, CT, CG>(p, t, kvh, blockIdx.y, k0 == 0 && kend == t.end, vref, m, l, o, ml, (float*)s_big);
 }
 
 // Joins the parts of a tile's columns: a wave a column

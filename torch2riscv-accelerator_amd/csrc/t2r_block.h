@@ -112,8 +112,10 @@ T2R_DEV Seq seq_of(const Ragged& g, int b) {
 
 // The piece'th of all sequences' pieces, a sequence having count(Seq) of them; in order, from the last one backwards, or the
 // later half backwards and then the earlier half forwards (a workgroup of the second round then does what its place in the
-// first left over, where pieces grow evenly: the tiles of a long prompt). Every wave of a workgroup finds it by itself, 64 sequences a step. Returns the piece's place in its sequence, -1 past
-// the last one.
+// first left over, where pieces grow evenly: the tiles of a long prompt). Every wave of a workgroup finds it by itself, 64
+// sequences a step. Returns the piece's place in its sequence, -1 past the last one. A sequence has fewer than kMaxRows
+// rows, so 64 of them count in 32 bits whatever `starts` holds; all of them may not.
+constexpr int kMaxRows = 1 << 24;
 enum { ORDER_FORWARDS = 0, ORDER_BACKWARDS = 1, ORDER_BOTH = 2 };
 template <int CTRL, int ROWS = 0xF> T2R_DEV int dpp_or_0(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false); }
 // sums over lanes 0 .. lane; the largest of a wave's lanes' values (none below 0), in every lane
@@ -137,16 +139,16 @@ T2R_DEV float wave_max0(float v) {
 }
 
 template <class F>
-T2R_DEV int find_piece(const Ragged& g, int piece, int order, F count, Seq* out) {
-  auto turn = [&](int total) {
+T2R_DEV int find_piece(const Ragged& g, long long piece, int order, F count, Seq* out) {
+  auto turn = [&](long long total) {
     if (order == ORDER_FORWARDS) return piece;
-    if (piece >= total) return -1;
-    const int half = order == ORDER_BOTH ? (total + 1) / 2 : total;
+    if (piece >= total) return -1LL;
+    const long long half = order == ORDER_BOTH ? (total + 1) / 2 : total;
     return piece < half ? total - 1 - piece : piece - half;
   };
   if (g.B == 1) {
     *out = seq_of(g, 0);
-    const int total = count(*out), t = turn(total);
+    const int total = count(*out), t = (int)turn(total);
     return t < total ? t : -1;
   }
   const int lane = threadIdx.x & 63;
@@ -161,22 +163,22 @@ T2R_DEV int find_piece(const Ragged& g, int piece, int order, F count, Seq* out)
   };
   int total = scan(0);
   if (order != ORDER_FORWARDS) {
-    int sum = total;
+    long long sum = total;
     for (int b0 = 64; b0 < g.B; b0 += 64) sum += scan(b0);
     piece = turn(sum);
     if (piece < 0) return -1;
     if (g.B > 64) total = scan(0);
   }
-  int base = 0;
+  long long base = 0;
   for (int b0 = 0;;) {
     if (piece < base + total) {
-      const int l = __builtin_ctzll(__ballot(base + s > piece));
+      const int l = __builtin_ctzll(__ballot(s > (int)(piece - base)));
       auto of = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
       out->b = b0 + l;
       out->r0 = of(q.r0);
       out->n = of(q.n);
       out->p0 = (long long)(((unsigned long long)(uint32_t)of((int)(q.p0 >> 32)) << 32) | (uint32_t)of((int)q.p0));
-      return piece - (base + of(s) - of(c));
+      return (int)(piece - base) - (of(s) - of(c));
     }
     base += total;
     b0 += 64;
@@ -316,7 +318,7 @@ __global__ __launch_bounds__(kBlkThreads) void k_blk_append(BlkRows x, Ragged g,
 }
 
 // Rows out of the cache, as the values that the codes stand for; zeros where the table holds no such position.
-template <class E, int NU>
+template <class E>
 __global__ __launch_bounds__(kBlkThreads) void k_blk_read(Ragged g, BlkCache c, E* k, E* v) {
   const int tid = threadIdx.x, head = blockIdx.y, hd = c.hd, lbs = c.lbs;
   const bool is_v = blockIdx.z != 0;
@@ -332,10 +334,7 @@ __global__ __launch_bounds__(kBlkThreads) void k_blk_read(Ragged g, BlkCache c, 
   const int8_t* tile = (is_v ? c.vc : c.kc) + at * c.tile_bytes();
   E* dst = (is_v ? v : k) + row * ld + (long long)head * hd;
   const int per = is_v ? hd : hd >> 4, units = is_v ? per << (lbs - 4) : per << lbs;
-#pragma unroll
-  for (int i = 0; i < NU; ++i) {
-    const int u = tid + i * kBlkThreads;
-    if (u >= units) break;
+  for (int u = tid; u < units; u += kBlkThreads) {
     const int a = u / per, b = u - a * per;
     const int from = is_v ? max(lo - a * 16, 0) : a >= lo ? 0 : 16, to = is_v ? min(hi - a * 16, 16) : a < hi ? 16 : 0;
     if (from >= to) continue;

@@ -14,6 +14,8 @@ using namespace t2r;
 
 namespace {
 
+constexpr long long kMaxGroups = (1 << 24) - 1;      // workgroups of 256 along x: a launch's threads count in 32 bits there
+
 inline int launched() { return hipGetLastError() == hipSuccess ? T2R_OK : T2R_EHIP; }
 inline long long cdiv(long long a, long long b) { return (a + b - 1) / b; }
 inline size_t elem_size(int dtype) { return dtype == T2R_F32 ? 4 : 2; }
@@ -49,7 +51,7 @@ long long blocks_entered(long long rows, long long B, int block) {
   return s + (x < x / block + s ? x : x / block + s);
 }
 
-// units of 16 values that a thread of the append and read kernels has (1, 2 or 4): 128 x 128 values are the most
+// units of 16 values that a thread of the append kernel has (1, 2 or 4): 128 x 128 values are the most
 int units_of(int hd, int block) {
   const int n = hd * block;
   return n <= 16 * kBlkThreads ? 1 : n <= 32 * kBlkThreads ? 2 : 4;
@@ -129,7 +131,7 @@ int t2r_kv_append_blk(const void* k, const void* v, int dtype, int64_t k_ld, int
   if (misaligned(k, elem_size(dtype)) || misaligned(v, elem_size(dtype)) || misaligned(starts, 4) || misaligned(lens, 4)) return T2R_EINVAL;
   BlkCache c;
   if (int rc = cache_args(kc, vc, ks, vs, n_blocks, block, Hk, hd, table, width, &c)) return rc;
-  if (B <= 0 || rows <= 0 || k_ld < (int64_t)Hk * hd || v_ld < (int64_t)Hk * hd) return T2R_ESHAPE;
+  if (B <= 0 || rows <= 0 || rows >= kMaxRows || k_ld < (int64_t)Hk * hd || v_ld < (int64_t)Hk * hd) return T2R_ESHAPE;
   const BlkRows x{k, v, k_ld, v_ld};
   const Ragged g{starts, lens, B, rows};
   const dim3 grid((unsigned)blocks_entered(rows, B, block), Hk, 2);
@@ -153,18 +155,14 @@ int t2r_kv_read_blk(const int8_t* kc, const int8_t* vc, const float* ks, const f
   if (misaligned(k, elem_size(dtype)) || misaligned(v, elem_size(dtype)) || misaligned(starts, 4) || misaligned(lens, 4)) return T2R_EINVAL;
   BlkCache c;
   if (int rc = cache_args(kc, vc, ks, vs, n_blocks, block, Hk, hd, table, width, &c)) return rc;
-  if (B <= 0 || rows <= 0) return T2R_ESHAPE;
+  if (B <= 0 || rows <= 0 || rows >= kMaxRows) return T2R_ESHAPE;
   const Ragged g{starts, lens, B, rows};
   const dim3 grid((unsigned)blocks_entered(rows, B, block), Hk, 2);
   return by_type(dtype, [&](auto e) {
     using E = decltype(e);
     const dim3 threads(kBlkThreads);
     const hipStream_t st = (hipStream_t)stream;
-    switch (units_of(hd, block)) {
-      case 1: launch((k_blk_read<E, 1>), grid, threads, 0, st, g, c, (E*)k, (E*)v); break;
-      case 2: launch((k_blk_read<E, 2>), grid, threads, 0, st, g, c, (E*)k, (E*)v); break;
-      default: launch((k_blk_read<E, 4>), grid, threads, 0, st, g, c, (E*)k, (E*)v); break;
-    }
+    launch(k_blk_read<E>, grid, threads, 0, st, g, c, (E*)k, (E*)v);
     return launched();
   });
 }
@@ -216,9 +214,9 @@ int t2r_attn_blk_prefill(const void* q, int dtype, int64_t q_ld, const int8_t* k
   BlkAttn p;
   std::memset(&p, 0, sizeof(p));
   if (int rc = cache_args(kc, vc, ks, vs, n_blocks, block, Hk, hd, table, width, &p.c)) return rc;
-  if (!attn_shape_ok(H, Hk) || B <= 0 || rows <= 0 || q_ld < (int64_t)H * hd || out_ld < (int64_t)H * hd) return T2R_ESHAPE;
+  if (!attn_shape_ok(H, Hk) || B <= 0 || rows <= 0 || rows >= kMaxRows || q_ld < (int64_t)H * hd || out_ld < (int64_t)H * hd) return T2R_ESHAPE;
   const Cut cut = rows_cut(B, rows, H, Hk, hd, block, width);
-  if (cut.nsplit > 65535 || (long long)cut.tiles * Hk > INT32_MAX) return T2R_ESHAPE;
+  if (cut.nsplit > 65535 || (long long)cut.tiles * Hk > kMaxGroups) return T2R_ESHAPE;
   const long long need = rows_ws(cut, Hk, hd);
   if (need > 0 && (!workspace || workspace_bytes < need || misaligned(workspace, 16))) return T2R_ENOMEM;
   p.q = q; p.q_ld = q_ld; p.out = out; p.out_ld = out_ld;
@@ -236,10 +234,10 @@ int t2r_attn_blk_prefill(const void* q, int dtype, int64_t q_ld, const int8_t* k
       if (hd <= 64) launch((k_blk_few<E, 64>), grid, block, 0, st, p);
       else launch((k_blk_few<E, 128>), grid, block, 0, st, p);
     } else if (cut.cols == 64) {
-      if (hd <= 64) launch((k_blk_tile<E, 64, 1, 2>), grid, block, 0, st, p);
-      else launch((k_blk_tile<E, 128, 1, 2>), grid, block, 0, st, p);
+      if (hd <= 64) launch((k_blk_tile<E, 64, 1>), grid, block, 0, st, p);
+      else launch((k_blk_tile<E, 128, 1>), grid, block, 0, st, p);
     } else {
-      launch((k_blk_tile<E, 64, 2, 2>), grid, block, 0, st, p);
+      launch((k_blk_tile<E, 64, 2>), grid, block, 0, st, p);
     }
     if (cut.nsplit > 1) launch(k_blk_rows_join<E>, dim3(cut.tiles * Hk, cut.cols / kBaWaves), block, 0, st, p, cut.cols);
     return launched();
@@ -262,7 +260,7 @@ int t2r_logprobs(const void* logits, int dtype, int64_t ld, const int32_t* token
   if (rows <= 0 || V <= 0 || ld < V) return T2R_ESHAPE;
   if (top < 0 || top > kLpMaxTop || top > V) return T2R_ERANGE;
   const Cut cut = lp_cut(rows, V);
-  if ((long long)rows * cut.nsplit > INT32_MAX) return T2R_ESHAPE;
+  if ((long long)rows * cut.nsplit > kMaxGroups) return T2R_ESHAPE;
   const long long need = t2r_logprobs_workspace_bytes(rows, V, top);
   if (need > 0 && (!workspace || workspace_bytes < need || misaligned(workspace, 16))) return T2R_ENOMEM;
   LpArgs p;
