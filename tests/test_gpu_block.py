@@ -486,6 +486,39 @@ def test_logprobs_odd_rows(env):
     assert ops.logprobs(put(torch, x))[0] is None
 
 
+@pytest.mark.parametrize("rows", [13, 1030])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_logprobs_over_spans(env, rows, dtype):
+    """A vocabulary of five whole spans of 8192 values and a rest, in a workgroup a span (few rows) or one for all: ranges
+    banned with -inf or the type's lowest value, the largest values in the first, a middle, the last span, many of them or
+    equal ones, rising and falling rows, a NaN and an infinity in later spans. The rows that differ are compared, and the last."""
+    torch, ops = env
+    rng = np.random.default_rng(19)
+    V, S, low = 5 * 8192 + 40, 8192, float(torch.finfo(torch.bfloat16).min)
+    x = (rng.standard_normal((13, V)) * 2).astype(F)
+    x[0, :S] = -np.inf
+    x[1, S:] = low
+    x[2, :3 * S] = low
+    x[3, 2 * S:3 * S] += 30
+    x[4, 5 * S:] += 30
+    x[5, :S] -= 40                                                     # all of the later spans beat the first
+    x[6] = np.arange(V) * 2.0 ** -9
+    x[7] = -np.arange(V) * 2.0 ** -9
+    x[8, 300::100] = 9                                                 # (more equal ones than candidates are held, over the spans)
+    x[9, 3 * S + 5] = np.nan
+    x[10, 5 * S + 39] = np.inf
+    x[11, S:2 * S] = -np.inf
+    x[11, 4 * S:] = -np.inf
+    x[11, 2 * S:4 * S] = low
+    full = np.concatenate([x, (rng.standard_normal((rows - 13, V))).astype(F)])
+    full, t = rounded(torch, full, dtype)
+    tokens = rng.integers(0, V, rows)
+    look = sorted({*range(13), rows - 1})
+    for top in (0, 5, 32):
+        got = ops.logprobs(t, i32(torch, tokens), top=top)
+        lp_check(torch, full[look].astype(np.float64), tuple(g[look] for g in got), tokens[look], top, 6)
+
+
 # ------------------------------------------------------------------ calls as programs make them
 def serving_step(torch, ops, c, w, qkv, starts, lens, H, hd, Hk, step):
     """Append, attend, a linear layer to logits, and the answers' log probabilities."""

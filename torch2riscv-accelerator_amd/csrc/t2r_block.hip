@@ -114,7 +114,7 @@ long long rows_ws(const Cut& c, int Hk, int hd) {
 
 // Parts of a logits row: as many as give the launch four workgroups a CU, each of whole spans
 Cut lp_cut(int rows, int V) {             // chunk: spans a part takes; nsplit: parts
-  const long long spans = cdiv(V, kLpSpan);
+  const long long spans = cdiv(V + (V >= kLpSpan ? 7LL : 0), kLpSpan);      // (spans begin at 16 bytes, up to 7 values early)
   const long long want = cdiv(1024, rows) < kLpMaxParts ? cdiv(1024, rows) : kLpMaxParts;
   const long long per = cdiv(spans, want < spans ? want : spans);
   return Cut{(int)per, (int)cdiv(spans, per), 0, 0};
@@ -257,7 +257,7 @@ int t2r_logprobs(const void* logits, int dtype, int64_t ld, const int32_t* token
   if (misaligned(logits, elem_size(dtype)) || misaligned(tokens, 4) || misaligned(logprob, 4) || misaligned(entropy, 4) ||
       misaligned(top_ids, 4) || misaligned(top_logprob, 4))
     return T2R_EINVAL;
-  if (rows <= 0 || V <= 0 || ld < V) return T2R_ESHAPE;
+  if (rows <= 0 || V <= 0 || V > INT32_MAX - 2 * kLpSpan || ld < V) return T2R_ESHAPE;
   if (top < 0 || top > kLpMaxTop || top > V) return T2R_ERANGE;
   const Cut cut = lp_cut(rows, V);
   if ((long long)rows * cut.nsplit > kMaxGroups) return T2R_ESHAPE;

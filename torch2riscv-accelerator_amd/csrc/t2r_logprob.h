@@ -10,9 +10,13 @@ namespace t2r {
 
 constexpr int kLpThreads = 256, kLpWaves = kLpThreads / 64, kLpPer = 32, kLpSpan = kLpThreads * kLpPer;
 constexpr int kLpMaxTop = 32;
-constexpr int kLpCand = 512;                 // candidates that a span's quick selection holds
+// Loads with candidates that wait for the next spans, at most: more make the selections, whose work grows with the square, the
+// dearer (24 / 64 / 200: 112 / 117 / 126 us for the top 20 of 2032 bf16 rows of 128256).
+constexpr int kLpMany = 24;
+constexpr int kLpKeys = 512;                 // keys that the quick selection holds
 constexpr int kLpMaxParts = 64;              // parts of a row
 constexpr float kLpNone = -__builtin_inff();
+constexpr float kLpSlack = 4.0f;
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
 // Sums run about c = F(m log2 e) in powers of two, l = sum 2^t and e = sum t 2^t with t = x log2 e - c, one fused step a
 // value; past this size, where x log2 e or c may overflow, t = (x - m) log2 e instead and c stands for m log2 e exactly.
@@ -25,8 +29,9 @@ T2R_DEV void lp_move(float m, float n, float* l, float* e) {
   if (fabsf(m) < kLpHuge && fabsf(n) < kLpHuge) d = m * kLog2e - n * kLog2e;
   if (*l == 0) return;                                                 // (d may be -inf)
   const float f = __builtin_amdgcn_exp2f(d);
-  *e = (*e + d * *l) * f;
-  *l *= f;
+  const float to = *l * f;                                             // (a NaN stays)
+  *e = f == 0 ? to : (*e + d * *l) * f;
+  *l = to;
 }
 
 struct LpArgs {
@@ -60,12 +65,14 @@ template <int CTRL> T2R_DEV float max_dpp(float x) {
 }
 
 struct LpLds {
-  unsigned long long best[2][kLpMaxTop];     // the largest so far, in order (0: none), before and after a span
-  unsigned long long cand[kLpCand];
-  float grp[2][kLpThreads / 4];
+  unsigned long long best[2][kLpMaxTop];     // the largest so far, in order (0: none), before and after a selection
+  unsigned long long key[kLpKeys];
+  int cand[kLpMany + kLpSpan / 4];           // loads with candidates: where they begin in the row
+  float grp[kLpThreads / 4];
   unsigned long long redk[kLpWaves];
-  float red[2][kLpWaves];
-  int n[2];
+  float red[3][kLpWaves];
+  int n[3];                                  // a span's loads with candidates, the next one's, those of the one before
+  int keys;
 };
 
 // What is told of a row: from m, l and e, and its largest keys in order.
@@ -89,155 +96,74 @@ T2R_DEV void lp_top(const LpArgs& p, int row, int place, unsigned long long k, f
 
 template <class E>
 __global__ __launch_bounds__(kLpThreads, 4) void k_lp_part(LpArgs p) {
-  constexpr int PER = 16 / sizeof(E), NL = kLpPer / PER;              // elements of a load, loads of a thread
+  constexpr int PER = 16 / sizeof(E), NL = kLpPer / PER;              // values of a load, loads of a thread
   struct __attribute__((packed, aligned(sizeof(E)))) Vec { v4i_t v; };
   __shared__ LpLds s;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int row = blockIdx.x / p.parts, part = blockIdx.x - row * p.parts, top = p.top, V = p.V;
   const E* x = (const E*)p.x + (long long)row * p.ld;
-  if (tid < 2 * kLpMaxTop) (&s.best[0][0])[tid] = 0;                         // (both rows: a part may hold fewer than top values)
-  if (tid == 0) s.n[0] = 0;
+  if (tid < 2 * kLpMaxTop) (&s.best[0][0])[tid] = 0;                   // (both rows: a part may hold fewer than top values)
+  if (tid < 3) s.n[tid] = 0;
+  if (tid == 0) s.keys = 0;
   int now = 0;                                                         // the row of s.best that holds
-  float m = kLpNone, l = 0, e = 0;                                     // of the part so far; l and e this thread's
-  Vec w[NL];
-  // a whole span's loads, issued a span ahead
+  // This thread's sums so far run about a value m of its own, no further than kLpSlack below its maximum: only the end brings
+  // the threads together, and few spans move it.
+  float m = kLpNone, l = 0, e = 0;
+  // Load i of a thread begins at place (i kLpThreads + tid) PER of its span. Spans of long rows begin `off` values before the
+  // row, so that whole ones are loaded at multiples of 16 bytes (odd rows of 49155 values took 46 us of loads and sums, even
+  // ones 40). A load over the row's beginning or end is moved inside; the values that are another load's too count as -inf
+  // then. Loads are issued a span ahead.
+  v4i_t w[NL];
+  const int off = V >= kLpSpan ? (int)((uintptr_t)x % 16 / sizeof(E)) : 0;
+  auto start_of = [&](int sp) { return ((long long)part * p.spans + sp) * kLpSpan - off; };
   auto fetch = [&](int sp) {
-    const long long i0 = ((long long)part * p.spans + sp) * kLpSpan;
-    if (sp < p.spans && i0 + kLpSpan <= V) {
+    const long long i0 = start_of(sp);
+    if (sp >= p.spans || i0 >= V) return;
+    if (i0 >= 0 && i0 + kLpSpan <= V) {
+      if (off == 0 && (uintptr_t)x % 16) {
 #pragma unroll
-      for (int i = 0; i < NL; ++i) w[i] = ((const Vec*)(x + i0 + i * kLpThreads * PER))[tid];
-    }
-  };
-  fetch(0);
-  for (int sp = 0; sp < p.spans; ++sp) {
-    const long long i0 = ((long long)part * p.spans + sp) * kLpSpan;
-    if (i0 >= V) break;
-    const int n = (int)min((long long)kLpSpan, V - i0), odd = sp & 1;
-    // Load i of a thread takes the PER values from place (i kLpThreads + tid) PER of the span on. In a span that the row's end
-    // cuts, loads past it are moved back to the row's last PER values; of those the first skip(i) lie before the thread's
-    // place (another load has them) and count as -inf.
-    const int lastv = n - PER;
-    // (the places are worked out anew in every span: kept over the loop they would take 60 registers more than there are)
-    int tq = tid;
-    asm volatile("" : "+v"(tq));
-    auto place = [&](int i) { return (i * kLpThreads + tq) * PER; };
-    auto skip = [&](int i) { return max(place(i) - lastv, 0); };
-    float v[kLpPer];
-    const bool whole = n == kLpSpan;
-    if (whole) {
+        for (int i = 0; i < NL; ++i) w[i] = ((const Vec*)(x + i0 + i * kLpThreads * PER))[tid].v;
+      } else {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) w[i] = ((const v4i_t*)(x + i0 + i * kLpThreads * PER))[tid];
+      }
     } else if (V >= PER) {
 #pragma unroll
-      for (int i = 0; i < NL; ++i) w[i] = *(const Vec*)(x + (i0 + min(place(i), lastv)));
+      for (int i = 0; i < NL; ++i) w[i] = ((const Vec*)(x + min(max(i0 + (i * kLpThreads + tid) * PER, 0LL), (long long)V - PER)))->v;
     } else {
       // a row of fewer values than a load takes: thread 0's first load, by hand, its values at the end
-      for (int i = 0; i < NL; ++i) w[i].v = v4i_t{0, 0, 0, 0};
+      for (int i = 0; i < NL; ++i) w[i] = v4i_t{0, 0, 0, 0};
       E* e0 = (E*)&w[0];
       for (int j = 0; j < PER; ++j)
         if (j >= PER - V) e0[j] = x[j - (PER - V)];
     }
-#pragma unroll
-    for (int i = 0; i < kLpPer; ++i) {
-      if constexpr (sizeof(E) == 4) v[i] = fv((uint32_t)w[i / PER].v[i % PER]);
-      else v[i] = widen(__builtin_bit_cast(E, (uint16_t)((uint32_t)w[i / PER].v[i % PER >> 1] >> (16 * (i & 1)))));
-    }
-    fetch(sp + 1);
-    uint32_t mine = ~0u;                                               // the values of its loads that are this thread's
-    if (!whole) {
-      mine = 0;
-#pragma unroll
-      for (int i = 0; i < NL; ++i) mine |= ((1u << PER) - 1) >> min(skip(i), PER) << min(skip(i), PER) << (i * PER);
-#pragma unroll
-      for (int i = 0; i < kLpPer; ++i) v[i] = mine >> i & 1 ? v[i] : kLpNone;
-    }
-    // value i again, from the cache: an index into registers would put them all into memory
-    auto key = [&](int i) {
-      const int at = place(i / PER) - (whole ? 0 : skip(i / PER)) + i % PER;
-      return lp_key(widen(x[i0 + at]), (uint32_t)(i0 + at));
-    };
-    float lm[NL], tm = kLpNone;                                        // the maxima of the loads, and of all of them
-#pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      lm[i] = v[i * PER];
-#pragma unroll
-      for (int j = 1; j < PER; ++j) lm[i] = fmaxf(lm[i], v[i * PER + j]);
-      tm = fmaxf(tm, lm[i]);
-    }
-    // the maxima of the 64 groups of 4 threads, to every wave: the span's maximum, and below the bound of its largest
-    const float gm = max_dpp<0x4E>(max_dpp<0xB1>(tm));
-    if ((tid & 3) == 0) s.grp[odd][tid >> 2] = gm;
-    __syncthreads();
-    const float g = s.grp[odd][lane];
-    float bm = max_dpp<0x121>(max_dpp<0x122>(max_dpp<0x124>(max_dpp<0x128>(g))));      // of 16 lanes
-    bm = fmaxf(bm, __shfl_xor(bm, 16));
-    bm = fmaxf(m, fmaxf(bm, __shfl_xor(bm, 32)));
-    if (bm > m) {                                                      // (uniform)
-      if (m != kLpNone) lp_move(m, bm, &l, &e);                        // (else both are 0, or NaN and stay that)
-      m = bm;
-    }
-    const float mu = m == kLpNone ? 0.0f : m;
-    float ls = 0;
-    if (!whole && !__any(mine != 0)) {
-      // (a wave that the row's last span leaves nothing)
-    } else if (fabsf(mu) < kLpHuge) {
-      const float c = mu * kLog2e;
-#pragma unroll
-      for (int i = 0; i < kLpPer; ++i) {
-        const float t = __builtin_fmaf(v[i], kLog2e, -c), q = __builtin_amdgcn_exp2f(t);
-        ls += q;
-        e = __builtin_fmaf(q, fmaxf(t, -200.0f), e);                   // (q is 0 there: -inf adds nothing)
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < kLpPer; ++i) {
-        const float t = (v[i] - mu) * kLog2e, q = __builtin_amdgcn_exp2f(t);
-        ls += q;
-        e = __builtin_fmaf(q, fmaxf(t, -200.0f), e);
-      }
-    }
-    l += ls;
-    if (top == 0) continue;
-    // A lower bound of the top-th largest value: the last of the best so far, or in the first span the top-th largest of the
-    // groups' maxima, to its upper 16 bits. What lies at or above it is a candidate: a few dozen of 8192 values as a rule.
-    uint32_t bound = (uint32_t)(s.best[now][top - 1] >> 32);
-    if (bound == 0) {
-      const uint32_t og = order_of(g);
-#pragma unroll
-      for (int bit = 31; bit >= 16; --bit) {
-        const uint32_t t = bound | (1u << bit);
-        bound = __popcll(__ballot(og >= t)) >= top ? t : bound;
-      }
-    }
-    const float least = order_value(max(bound, kOrderNone));
-    if (tid == 0) s.n[odd ^ 1] = 0;
-    const bool nan = ls != ls;                                         // (a NaN among the values, or an infinity)
-    if (tm >= least || nan) {
-      uint32_t set = 0;
-#pragma unroll
-      for (int i = 0; i < NL; ++i)
-        if (lm[i] >= least) {
-#pragma unroll
-          for (int j = 0; j < PER; ++j) set |= v[i * PER + j] >= least ? 1u << (i * PER + j) : 0u;
-        }
-      if (nan) {
-#pragma unroll
-        for (int i = 0; i < kLpPer; ++i) set |= v[i] != v[i] ? 1u << i : 0u;
-      }
-      set &= mine;
-      // one place for all of a thread's (an atomic and its wait for each took 90 us of 190 in 2032 rows of 49155)
-      int c = set ? atomicAdd(&s.n[odd], __popc(set)) : 0;
-      for (; set != 0; set &= set - 1, ++c)
-        if (c < kLpCand) s.cand[c] = key(__builtin_ctz(set));
+  };
+  // The candidates in the first n noted loads, and what was best, into the best: a key's rank is the number of larger ones (keys
+  // differ: their indices do; 0 is none).
+  uint32_t bound = 0;                                                  // of a candidate's order from below
+  auto value_key = [&](int c) {                                        // value c of the noted loads
+    const int i = s.cand[c / PER] + c % PER;
+    if (i < 0 || i >= V) return 0ull;
+    const unsigned long long k = lp_key(widen(x[i]), (uint32_t)i);
+    return (uint32_t)(k >> 32) >= bound ? k : 0ull;
+  };
+  auto settle = [&](int n) {
+    if (n == 0) return;
+    for (int c = tid; c < n * PER; c += kLpThreads) {
+      const unsigned long long k = value_key(c);
+      if (k == 0) continue;
+      const int at = atomicAdd(&s.keys, 1);
+      if (at < kLpKeys) s.key[at] = k;
     }
     __syncthreads();
-    int nc = s.n[odd];
-    if (nc > kLpCand) {
-      // many equal values: the span's largest keys one by one
+    int nk = s.keys;
+    if (nk > kLpKeys) {
+      // too many (equal values, say): the largest one by one
       unsigned long long below = ~0ull;
-      for (int c = 0; c < top; ++c) {
+      for (nk = 0; nk < top; ++nk) {
         unsigned long long b = 0;
-#pragma unroll 4
-        for (int i = 0; i < kLpPer; ++i) {
-          const unsigned long long k = mine >> i & 1 ? key(i) : 0;
+        for (int c = tid; c < n * PER; c += kLpThreads) {
+          const unsigned long long k = value_key(c);
           b = k < below && k > b ? k : b;
         }
 #pragma unroll
@@ -250,43 +176,145 @@ __global__ __launch_bounds__(kLpThreads, 4) void k_lp_part(LpArgs p) {
 #pragma unroll
         for (int w = 0; w < kLpWaves; ++w) b = s.redk[w] > b ? s.redk[w] : b;
         below = b;
-        if (tid == 0) s.cand[c] = b;
+        if (tid == 0) s.key[nk] = b;
         __syncthreads();
       }
-      nc = top;
     }
-    if (nc > 0) {                                                      // (uniform)
-      // each key's rank is the number of larger ones (keys differ: their indices do; 0 is none)
-      const unsigned long long* was = s.best[now];
-      unsigned long long* next = s.best[now ^ 1];
-      for (int i = tid; i < nc + top; i += kLpThreads) {
-        const unsigned long long k = i < nc ? s.cand[i] : was[i - nc];
-        int r = 0;
+    const unsigned long long* was = s.best[now];
+    unsigned long long* next = s.best[now ^ 1];
+    for (int i = tid; i < nk + top; i += kLpThreads) {
+      const unsigned long long k = i < nk ? s.key[i] : was[i - nk];
+      int r = 0;
 #pragma unroll 8
-        for (int j = 0; j < nc; ++j) r += s.cand[j] > k;
+      for (int j = 0; j < nk; ++j) r += s.key[j] > k;
 #pragma unroll 4
-        for (int j = 0; j < top; ++j) r += was[j] > k;
-        if (k != 0 && r < top) next[r] = k;
+      for (int j = 0; j < top; ++j) r += was[j] > k;
+      if (k != 0 && r < top) next[r] = k;
+    }
+    now ^= 1;
+    if (tid == 0) s.keys = 0;
+    __syncthreads();
+    bound = max(bound, (uint32_t)(s.best[now][top - 1] >> 32));
+  };
+  int noted = 0;                                                       // loads of earlier spans
+  fetch(0);
+  for (int sp = 0; sp < p.spans; ++sp) {
+    const long long i0 = start_of(sp);
+    if (i0 >= V) break;
+    const int turn = sp % 3;
+    const bool whole = i0 >= 0 && i0 + kLpSpan <= V;
+    uint32_t mine = ~0u;                                               // the values of its loads that are this thread's
+    if (!whole) {
+      mine = 0;
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int at = (i * kLpThreads + tid) * PER;
+        const int before = (int)min(max(-i0 - at, 0LL), (long long)PER), past = (int)min(max(i0 + at - (V - PER), 0LL), (long long)PER);
+        mine |= ((1u << PER) - 1) >> before >> past << past << (i * PER);
       }
-      now ^= 1;
+    }
+    const bool some = whole || __any(mine != 0);                       // (the row's last span may leave a wave nothing)
+    float v[kLpPer], lm[NL], tm = kLpNone, ls = 0;                     // the maxima of the loads, and of all of them
+    if (some) {
+#pragma unroll
+      for (int i = 0; i < kLpPer; ++i) {
+        if constexpr (sizeof(E) == 4) v[i] = fv((uint32_t)w[i / PER][i % PER]);
+        else v[i] = widen(__builtin_bit_cast(E, (uint16_t)((uint32_t)w[i / PER][i % PER >> 1] >> (16 * (i & 1)))));
+      }
+      fetch(sp + 1);
+      if (!whole && __any(mine != ~0u)) {
+#pragma unroll
+        for (int i = 0; i < kLpPer; ++i) v[i] = mine >> i & 1 ? v[i] : kLpNone;
+      }
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        lm[i] = v[i * PER];
+#pragma unroll
+        for (int j = 1; j < PER; ++j) lm[i] = fmaxf(lm[i], v[i * PER + j]);
+        tm = fmaxf(tm, lm[i]);
+      }
+      if (tm > m + kLpSlack) {
+        if (m != kLpNone) lp_move(m, tm, &l, &e);                      // (else both are 0, or NaN and stay that)
+        m = tm;
+      }
+      const float mu = m == kLpNone ? 0.0f : m;
+      if (fabsf(mu) < kLpHuge) {
+        const float c = mu * kLog2e;
+#pragma unroll
+        for (int i = 0; i < kLpPer; ++i) {
+          const float t = __builtin_fmaf(v[i], kLog2e, -c), q = __builtin_amdgcn_exp2f(t);
+          ls += q;
+          e = __builtin_fmaf(q, fmaxf(t, -200.0f), e);                 // (q is 0 there: -inf adds nothing)
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kLpPer; ++i) {
+          const float t = (v[i] - mu) * kLog2e, q = __builtin_amdgcn_exp2f(t);
+          ls += q;
+          e = __builtin_fmaf(q, fmaxf(t, -200.0f), e);
+        }
+      }
+      l += ls;
+    }
+    if (top == 0) continue;
+    // A lower bound of the top-th largest value: the last of the best so far, or before the first selection the top-th largest
+    // of the first span's maxima of 64 groups of 4 threads, to its upper 16 bits. Loads that hold something at or above it, a
+    // dozen of a span's 1024 or 2048 as a rule, are noted, and selected from at the end or once they are many.
+    if (sp == 0) {
+      const float gm = max_dpp<0x4E>(max_dpp<0xB1>(tm));
+      if ((tid & 3) == 0) s.grp[tid >> 2] = gm;
+      __syncthreads();
+      const uint32_t og = order_of(s.grp[lane]);
+#pragma unroll
+      for (int bit = 31; bit >= 16; --bit) {
+        const uint32_t t = bound | (1u << bit);
+        bound = __popcll(__ballot(og >= t)) >= top ? t : bound;
+      }
+      bound = max(bound, kOrderNone);
+    }
+    const float least = order_value(bound);
+    if (tid == 0) s.n[(sp + 1) % 3] = 0;                               // (last read two spans ago)
+    const bool nan = ls != ls;                                         // (a NaN among the values, or an infinity)
+    if (some && (tm >= least || nan)) {
+      int set = 0;
+#pragma unroll
+      for (int i = 0; i < NL; ++i) set |= lm[i] >= least || nan ? 1 << i : 0;
+      // one place for all of a thread's (an atomic and its wait for each value took 90 us of 190 in 2032 rows of 49155)
+      for (int c = noted + atomicAdd(&s.n[turn], __popc(set)); set != 0; set &= set - 1, ++c)
+        s.cand[c] = (int)i0 + (__builtin_ctz(set) * kLpThreads + tid) * PER;
+    }
+    __syncthreads();
+    noted += s.n[turn];
+    if (noted > kLpMany || sp + 1 == p.spans || i0 + kLpSpan >= V) {
+      settle(noted);
+      noted = 0;
     }
   }
-  // the sums over the threads
+  // the sums over the threads, about the largest m
+  float all = m;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor(all, o));
+  if (lane == 0) s.red[0][wave] = all;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kLpWaves; ++w) all = fmaxf(all, s.red[0][w]);
+  if (l == l) lp_move(m, all, &l, &e);
+  m = all;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     l += __shfl_xor(l, o);
     e += __shfl_xor(e, o);
   }
   if (lane == 0) {
-    s.red[0][wave] = l;
-    s.red[1][wave] = e;
+    s.red[1][wave] = l;
+    s.red[2][wave] = e;
   }
   __syncthreads();
   l = e = 0;
 #pragma unroll
   for (int w = 0; w < kLpWaves; ++w) {
-    l += s.red[0][w];
-    e += s.red[1][w];
+    l += s.red[1][w];
+    e += s.red[2][w];
   }
   if (p.parts == 1) {
     float lse;
