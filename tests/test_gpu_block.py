@@ -462,6 +462,26 @@ def test_logprobs(env, rows, V, top, dtype):
     lp_check(torch, x, ops.logprobs(t, i32(torch, tokens), top=top), tokens, top, 8)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("V", [7, 8191, 8192, 8193, 8200, 16383, 16392])
+def test_logprobs_starts_and_ends(env, V, dtype):
+    """Rows at every alignment, around whole spans; the largest value first, last and at a span's ends."""
+    torch, ops = env
+    rng = np.random.default_rng(V)
+    big, wide = rounded(torch, rng.standard_normal((9, V + 13)) * 2, dtype)
+    for off in range(8):
+        x, t = big[:, off:off + V].copy(), wide[:, off:off + V].clone()
+        hot = [0, V - 1, min(8191, V - 1), min(8192, V - 1), min(8192 - off, V - 1), max(V - 8, 0), V // 2, 1, 6]
+        x[np.arange(9), hot] = 11
+        held = torch.empty_like(wide)
+        held.fill_(float("nan"))                                       # (what lies beside the rows)
+        held[:, off:off + V] = t
+        held[torch.arange(9), off + torch.tensor(hot)] = 11
+        got = ops.logprobs(held[:, off:off + V], i32(torch, hot), top=min(V, 6))
+        lp_check(torch, x.astype(np.float64), got, np.asarray(hot), min(V, 6), 4)
+        assert got[2][:, 0].tolist() == hot
+
+
 def test_logprobs_odd_rows(env):
     """Banned values (-inf, the type's lowest), rows of nothing, of one value, of equal values, rising rows (every span beats
     the one before), NaN and +inf, tokens outside the vocabulary, -0 against +0."""
@@ -590,6 +610,101 @@ def test_two_graphs_on_another_stream(env):
             for a, b in zip(c.dev, twin[i]):
                 assert torch.equal(a, b)
             ln += 1
+
+
+def test_graph_of_ragged_rows(env):
+    """Turns and drafts captured with their appends (keys cut into parts, and whole), replayed while lengths and rows change."""
+    torch, ops = env
+    rng = np.random.default_rng(20)
+    H, Hk, hd = 8, 2, 64
+    for news, lens, width in (([5, 3], [900, 2500], 64), ([300, 180, 0], [400, 1300, 0], 64), ([700, 700], [900, 1500], 32)):
+        c = Both(torch, ops, rng, lens, Hk, hd, 64, width=width).fill(rng).send()
+        rows = sum(news)
+        st, ln, out = i32(torch, np.concatenate([[0], np.cumsum(news)])), i32(torch, lens), None
+        x = put(torch, rng.standard_normal((rows, (H + 2 * Hk) * hd)).astype(F))
+        k, v, q = x[:, H * hd:(H + Hk) * hd], x[:, (H + Hk) * hd:], x[:, :H * hd]
+
+        def turn(cache):
+            ops.kv_append_block(k, v, *cache, st, ln)
+            return ops.attention_block_prefill(q, *cache, st, ln, H)
+
+        twin = [t.clone() for t in c.dev]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            turn([t.clone() for t in c.dev])
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            out = turn(c.dev)
+        for _ in range(3):
+            x.copy_(put(torch, rng.standard_normal(tuple(x.shape)).astype(F)))
+            g.replay()
+            want = turn(twin)
+            torch.cuda.synchronize()
+            assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(c.dev, twin))
+            ln.sub_(7).clamp_(min=0)
+
+
+def test_calls_on_two_streams_at_once(env):
+    """Reads of one cache from two streams, without a wait between them."""
+    torch, ops = env
+    rng = np.random.default_rng(21)
+    H, Hk, hd = 16, 4, 128
+    lens = [3000, 90, 700]
+    c = Both(torch, ops, rng, lens, Hk, hd, 64).fill(rng).send()
+    xs = [put(torch, rng.standard_normal((3, H * hd)).astype(F)) for _ in range(2)]
+    ys = [put(torch, rng.standard_normal((120, H * hd)).astype(F)) for _ in range(2)]
+    zs = [put(torch, rng.standard_normal((9, 40000)).astype(F)) for _ in range(2)]
+    st = i32(torch, [0, 60, 100, 120])
+
+    def calls(i):
+        return (ops.attention_block(xs[i], *c.dev, c.lens_d, H), ops.attention_block_prefill(ys[i], *c.dev, st, c.lens_d, H),
+                *ops.logprobs(zs[i], top=9)[1:])
+
+    want = [calls(0), calls(1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(6):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((i, calls(i)))
+    torch.cuda.synchronize()
+    for i, g in got:
+        assert all(torch.equal(a, b) for a, b in zip(g, want[i]))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_result_in_the_query_s_place(env, dtype):
+    """The C entry points with out = q, whose rows lie apart: the same values as in a place of their own, and what lies between
+    the rows as it was."""
+    torch, ops = env
+    from t2r_amd import abi
+    rng = np.random.default_rng(22)
+    H, Hk, hd, block = 8, 2, 64, 64
+    code = {"f32": abi.T2R_F32, "bf16": abi.T2R_BF16}[dtype]
+    s = torch.cuda.current_stream().cuda_stream
+    for lens, news in (([300, 1], None), ([5000, 700], None), ([300, 90], [300, 17]), ([4000, 900], [6, 2]), ([2000, 0, 40], [1500, 0, 3])):
+        c = Both(torch, ops, rng, lens, Hk, hd, block).fill(rng).send()
+        rows, B = sum(news or [1] * len(lens)), len(lens)
+        _, t = rounded(torch, rng.standard_normal((rows, H * hd + 8)), dtype)
+        q = t[:, :H * hd]
+        st = i32(torch, np.concatenate([[0], np.cumsum(news)])) if news else None
+        want = ops.attention_block_prefill(q, *c.dev, st, c.lens_d, H) if news else ops.attention_block(q, *c.dev, c.lens_d, H)
+        kc, vc, ks, vs, table = c.dev
+        n, width = kc.shape[0], table.shape[1]
+        need = abi.load().t2r_attn_blk_workspace_bytes(B, rows if news else 0, H, Hk, hd, block, width, code)
+        ws = torch.empty(max(need, 16), dtype=torch.uint8, device="cuda:0")
+        beside = t[:, H * hd:].clone()
+        head = (t.data_ptr(), code, t.stride(0), kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), n, block, Hk, hd, table.data_ptr(), width)
+        tail = (H, 1 / math.sqrt(hd), t.data_ptr(), t.stride(0), ws.data_ptr(), need, s)
+        if news:
+            abi.call("t2r_attn_blk_prefill", *head, st.data_ptr(), c.lens_d.data_ptr(), B, rows, *tail)
+        else:
+            abi.call("t2r_attn_blk_decode", *head, c.lens_d.data_ptr(), B, *tail)
+        torch.cuda.synchronize()
+        assert torch.equal(t[:, :H * hd], want) and torch.equal(t[:, H * hd:], beside)
 
 
 def test_same_bits_every_time(env):

@@ -145,6 +145,11 @@ T2R_DEV float seg_scales(BaSeg& sg, const BlkCache& c, int blk, int head, int n,
 // A workgroup takes `chunk` keys of one (sequence, KV head) and up to HW of its query heads, its four waves every fourth
 // 64 of them. 16 x 16 x 32 MFMA: columns 0 .. HW - 1 are the heads; with fp32 rows columns 8 .. 15 hold their low
 // pieces, so that one product serves both and the columns are added afterwards.
+//
+// Every code is needed once, so the codes go from memory into the waves' registers, a step ahead, and never through LDS; the
+// loads of a step are 64 tokens' whole rows. Long caches are bound by memory: 32 sequences of 8192 tokens, 8 KV heads of 128,
+// 5.4 TB/s; of 1021 .. 8192 tokens 63 us (4.8 TB/s: the longest sequences end alone) and 4.3 for the join. Short ones are a
+// chain of length, table, scales, codes and products: one sequence of 96 tokens 4.5 us, of 8101 5.9 and 4.4.
 template <class E> struct Pieces { static constexpr int kN = sizeof(E) == 4 ? 2 : 1, kHeads = 16 / kN; };
 
 template <class E, int HD>
@@ -392,7 +397,7 @@ T2R_DEV void join_store(const BlkAttn& p, E* out, const float* x, float l, bool 
   out[d + 1] = narrow<E>(x[1] * inv);
 }
 
-// a workgroup per (head, sequence)
+// a workgroup per (head, sequence); 4.3 us, 3.3 of them an empty kernel's
 template <class E>
 __global__ __launch_bounds__(kBaThreads) void k_blk_step_join(BlkAttn p) {
   __shared__ float s_x[kBaWaves][64][2];
@@ -419,11 +424,17 @@ __global__ __launch_bounds__(kBaThreads) void k_blk_step_join(BlkAttn p) {
 // `chunk` of its keys where few rows meet long caches). 32 x 32 x 16 MFMA.
 //
 // k_blk_few: 32 columns. The four waves take every fourth 32 keys, each loading and converting its codes by itself: nothing
-// is shared but the columns, and no barrier stands in the loop.
+// is shared but the columns, and no barrier stands in the loop. 8 rows of each of four sequences over 5003 .. 8100 positions,
+// 32 heads of 64: 17.6 us in parts of 512 keys, of which a part's beginning and end are half, and 4.9 for the join.
 // k_blk_tile: 32 CT CG columns, CG groups of 32 CT for the waves; KG = 4 / CG waves of a group take the stage's 32 KG keys.
 // The workgroup loads a stage's codes together (a stage ahead), converts them once into LDS, in the MFMA operands' order,
 // two stages in turn with one barrier each. The conversion is as much vector work as the softmax of 32 columns (160
-// instructions of 32 keys at head dim 128 against 180), so CG waves share it.
+// instructions of 32 keys at head dim 128 against 180), so CG waves share it. Measured: one prompt of 2032 rows, 16 heads of 128
+// in fp32, 54.6 us (310 TFLOP/s of the formula's, twice that of fp16 products, q and p being two pieces); seven prompts and
+// turns in bf16, 32 heads of 64, 76 us (475 TFLOP/s). The last tiles of a long prompt set the time, 32 stages of 1.25 us after
+// 7 us before and after; in a wave the products of a stage (2 x 512 cycles at head dim 128 in fp32) and its 900 cycles of
+// softmax, conversions and LDS traffic add up, and the second workgroup of the CU hides little of the sum. More waves a
+// workgroup, a second stage in flight in registers and tiles cut along their keys all came out slower.
 struct Tile {
   Seq s;
   int t, i0, rows;          // tile t of sequence s: its rows i0 .. i0 + rows - 1

@@ -228,8 +228,12 @@ T2R_DEV uint32_t byte_mask(int i, int from, int to) {
 }
 
 // Rows into the cache: a workgroup takes one (block, KV head) of K or of V that rows enter: their maximum, the block's
-// new scale, the codes, and the block's older codes where the scale grew. A thread has NU units of 16 values, which stay in
-// registers between the two: K (token, 16 channels), V (channel, 16 tokens: lanes along the channels).
+// new scale, the codes, and the block's older codes where the scale grew. No other workgroup needs that scale, so one pass and
+// one launch do. A thread has NU units of 16 values, which stay in registers between the maximum and the codes: K (token,
+// 16 channels), V (channel, 16 tokens: lanes along the channels, so that loads are whole lines and a store is 16 codes).
+// Reads the rows, writes a byte a value. A call of few rows is a launch and one chain of loads (16 sequences of 8 heads of 64,
+// a row each: 5.3 us, 3.3 of them an empty kernel's); a prompt of 2032 rows of 8 heads of 128 in fp32 takes 11.5 us (1.8 TB/s
+// of 20.8 MB, 508 workgroups: loads, maximum, codes and stores follow each other in each, and all run at once).
 template <class E, int NU>
 __global__ __launch_bounds__(kBlkThreads) void k_blk_append(BlkRows x, Ragged g, BlkCache c) {
   __shared__ float red[kBlkThreads / 64];
@@ -317,7 +321,8 @@ __global__ __launch_bounds__(kBlkThreads) void k_blk_append(BlkRows x, Ragged g,
   if (tid == 0) *scale = now;
 }
 
-// Rows out of the cache, as the values that the codes stand for; zeros where the table holds no such position.
+// Rows out of the cache, as the values that the codes stand for; zeros where the table holds no such position. The same
+// pieces as above, the other way. 2032 rows of 8 heads of 128 to fp32: 8.9 us (2.3 TB/s); single rows 4.6 us.
 template <class E>
 __global__ __launch_bounds__(kBlkThreads) void k_blk_read(Ragged g, BlkCache c, E* k, E* v) {
   const int tid = threadIdx.x, head = blockIdx.y, hd = c.hd, lbs = c.lbs;

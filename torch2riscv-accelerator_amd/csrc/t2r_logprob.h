@@ -1,8 +1,13 @@
 // Log probabilities of logits rows: for x[V] with m = max x and l = sum exp(x - m),
 //   log p(t) = x[t] - (m + ln l),   entropy = ln l - sum (x - m) exp(x - m) / l,
 // and the `top` largest values with their indices (descending, the lower index first on ties, a NaN before everything).
-// The logits are read once: a workgroup takes parts of kLpSpan values of a row into registers and works out their maximum,
-// sums and largest values there; k_lp_join joins a row's parts.
+// The logits are read once: a workgroup takes spans of kLpSpan values of a row into registers, the next one's loads in flight,
+// and works out their maxima and sums there; k_lp_join joins a row's parts.
+//
+// fp32 logits are bound by memory (1024 rows of 151936, top 20: 116 us, 5.4 TB/s), 16-bit ones by the vector units: six
+// instructions a value, one of them an exponential that counts four times, and what a span needs besides. 2032 rows of 49155:
+// 52 us with the top 5 (3.8 TB/s), 43 without; of 128256: 112 us with the top 20 (4.6), 98 without. Few rows: 16 of 128256
+// 7.0 us and 6.6 for the join, an empty kernel taking 3.3.
 #pragma once
 #include "t2r_block.h"
 
@@ -56,12 +61,29 @@ T2R_DEV uint32_t order_of(float x) {
 T2R_DEV float order_value(uint32_t o) { return o == 0xFFFFFFFFu ? fv(kQNaN) : fv(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o); }
 T2R_DEV unsigned long long lp_key(float x, uint32_t i) { return ((unsigned long long)order_of(x) << 32) | (uint32_t)~i; }
 T2R_DEV float key_value(unsigned long long k) { return order_value((uint32_t)(k >> 32)); }
-T2R_DEV unsigned long long shfl_key(unsigned long long k, int from_xor) {
-  const uint32_t lo = __shfl_xor((int)(uint32_t)k, from_xor), hi = __shfl_xor((int)(uint32_t)(k >> 32), from_xor);
-  return ((unsigned long long)hi << 32) | lo;
+// f over the wave's values, to every lane (f needs no order)
+template <class F> T2R_DEV float wave_all(float x, F f) {
+  x = f(x, dpp_f<kDppXor1>(x));
+  x = f(x, dpp_f<kDppXor2>(x));
+  x = f(x, dpp_f<kDppHalfMirror>(x));
+  x = f(x, dpp_f<kDppMirror>(x));
+  auto of = [&](int lane) { return fv((uint32_t)__builtin_amdgcn_readlane((int)fb(x), lane)); };
+  return f(f(of(0), of(16)), f(of(32), of(48)));
 }
-template <int CTRL> T2R_DEV float max_dpp(float x) {
-  return fmaxf(x, fv((uint32_t)__builtin_amdgcn_update_dpp(0, (int)fb(x), CTRL, 0xF, 0xF, false)));
+T2R_DEV float wave_top(float x) { return wave_all(x, [](float a, float b) { return fmaxf(a, b); }); }
+T2R_DEV float wave_total(float x) { return wave_all(x, [](float a, float b) { return a + b; }); }
+// the largest key of the wave, to every lane
+template <int CTRL> T2R_DEV unsigned long long key_dpp(unsigned long long k) {
+  const unsigned long long o = ((unsigned long long)(uint32_t)dpp_i<CTRL>((int)(k >> 32)) << 32) | (uint32_t)dpp_i<CTRL>((int)(uint32_t)k);
+  return o > k ? o : k;
+}
+T2R_DEV unsigned long long wave_key(unsigned long long k) {
+  k = key_dpp<kDppMirror>(key_dpp<kDppHalfMirror>(key_dpp<kDppXor2>(key_dpp<kDppXor1>(k))));
+  auto of = [&](int lane) {
+    return ((unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(k >> 32), lane) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)k, lane);
+  };
+  const unsigned long long a = max(of(0), of(16)), b = max(of(32), of(48));
+  return max(a, b);
 }
 
 struct LpLds {
@@ -110,8 +132,8 @@ __global__ __launch_bounds__(kLpThreads, 4) void k_lp_part(LpArgs p) {
   // the threads together, and few spans move it.
   float m = kLpNone, l = 0, e = 0;
   // Load i of a thread begins at place (i kLpThreads + tid) PER of its span. Spans of long rows begin `off` values before the
-  // row, so that whole ones are loaded at multiples of 16 bytes (odd rows of 49155 values took 46 us of loads and sums, even
-  // ones 40). A load over the row's beginning or end is moved inside; the values that are another load's too count as -inf
+  // row, so that whole ones are loaded at multiples of 16 bytes (odd rows of 49155 values took 46 us of loads and sums, 43
+  // so). A load over the row's beginning or end is moved inside; the values that are another load's too count as -inf
   // then. Loads are issued a span ahead.
   v4i_t w[NL];
   const int off = V >= kLpSpan ? (int)((uintptr_t)x % 16 / sizeof(E)) : 0;
@@ -166,11 +188,7 @@ __global__ __launch_bounds__(kLpThreads, 4) void k_lp_part(LpArgs p) {
           const unsigned long long k = value_key(c);
           b = k < below && k > b ? k : b;
         }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-          const unsigned long long k = shfl_key(b, o);
-          b = k > b ? k : b;
-        }
+        b = wave_key(b);
         if (lane == 0) s.redk[wave] = b;
         __syncthreads();
 #pragma unroll
@@ -261,7 +279,8 @@ __global__ __launch_bounds__(kLpThreads, 4) void k_lp_part(LpArgs p) {
     // of the first span's maxima of 64 groups of 4 threads, to its upper 16 bits. Loads that hold something at or above it, a
     // dozen of a span's 1024 or 2048 as a rule, are noted, and selected from at the end or once they are many.
     if (sp == 0) {
-      const float gm = max_dpp<0x4E>(max_dpp<0xB1>(tm));
+      float gm = fmaxf(tm, dpp_f<kDppXor1>(tm));
+      gm = fmaxf(gm, dpp_f<kDppXor2>(gm));
       if ((tid & 3) == 0) s.grp[tid >> 2] = gm;
       __syncthreads();
       const uint32_t og = order_of(s.grp[lane]);
@@ -291,20 +310,15 @@ __global__ __launch_bounds__(kLpThreads, 4) void k_lp_part(LpArgs p) {
     }
   }
   // the sums over the threads, about the largest m
-  float all = m;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor(all, o));
+  float all = wave_top(m);
   if (lane == 0) s.red[0][wave] = all;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kLpWaves; ++w) all = fmaxf(all, s.red[0][w]);
   if (l == l) lp_move(m, all, &l, &e);
   m = all;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    l += __shfl_xor(l, o);
-    e += __shfl_xor(e, o);
-  }
+  l = wave_total(l);
+  e = wave_total(e);
   if (lane == 0) {
     s.red[1][wave] = l;
     s.red[2][wave] = e;
@@ -349,20 +363,12 @@ __global__ __launch_bounds__(kLpThreads) void k_lp_join(LpArgs p) {
     if (top > 0) last = from[lane * top + top - 1];
   }
   if (tid == 0) s_n = 0;
-  float m = sum[0];
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    m = fmaxf(m, __shfl_xor(m, o));
-    const unsigned long long k = shfl_key(last, o);
-    last = k > last ? k : last;
-  }
+  const float m = wave_top(sum[0]);
+  last = wave_key(last);
   float l = sum[1], e = sum[2];
   if (l == l) lp_move(sum[0], m, &l, &e);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    l += __shfl_xor(l, o);
-    e += __shfl_xor(e, o);
-  }
+  l = wave_total(l);
+  e = wave_total(e);
   float lse;
   lp_sums(p, row, xt, m, l, e, &lse);
   if (top == 0) return;
