@@ -238,6 +238,7 @@ ROWS = [
     (4, 2, 16, 16, [100], [2500], None),
     (7, 7, 112, 64, [31], [31], None),
     (20, 2, 128, 32, [17], [300], None),
+    (8, 2, 64, 64, [50, 0, 1, 0, 0, 2, 0, 0], [700, 5, 1, 0, 9, 2000, 3, 3], 64),      # (few rows in all, but not of the first)
 ]
 
 

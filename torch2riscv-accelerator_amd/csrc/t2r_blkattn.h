@@ -356,12 +356,16 @@ __global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_step(BlkAt
   }
 }
 
-// Joins the parts of a row: their sums, moved to the largest of their maxima. NWV waves take every NWV-th part each, a lane
-// two channels; what a wave has comes back in *x (and the weights' sum, the same in every wave). The parts' maxima are read
-// 64 at a time, a lane each; the sums' loads wait for nothing.
+// Joins the parts of a row: their sums, moved to the largest of their maxima. NWV waves of the workgroup take every NWV-th part
+// each, a lane two channels; what the row's first wave has in *x is the row (and the weights' sum, the same in every wave, comes
+// back). The parts' maxima are read 64 at a time, a lane each; the sums' loads wait for nothing. A wave has eight parts' sums
+// in flight, and eight more cost a memory's latency: from kJoinWide parts on a row is worth four waves (32 columns of 32
+// heads in 13 / 32 parts: 6.5 / 9.4 us with a wave each).
+constexpr int kJoinWide = 9;
 template <int NWV>
-T2R_DEV float join_parts(const BlkAttn& p, long long at, int parts, int wave, float (*x)[2]) {
-  const int lane = threadIdx.x & 63, hd = p.c.hd, d = min(2 * lane, hd - 2);
+T2R_DEV float join_parts(const BlkAttn& p, long long at, int parts, float (*x)[2]) {
+  __shared__ float s_x[NWV > 1 ? kBaWaves : 1][64][2];
+  const int lane = threadIdx.x & 63, hd = p.c.hd, d = min(2 * lane, hd - 2), wave = NWV > 1 ? wave_index() : 0;
   typedef float v2f_t __attribute__((ext_vector_type(2)));
   const v2f_t* ml = (const v2f_t*)p.ws_ml + at;
   float mm = kNegInf;
@@ -385,6 +389,16 @@ T2R_DEV float join_parts(const BlkAttn& p, long long at, int parts, int wave, fl
   for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
   (*x)[0] = y[0];
   (*x)[1] = y[1];
+  if constexpr (NWV > 1) {
+    s_x[wave][lane][0] = y[0];
+    s_x[wave][lane][1] = y[1];
+    __syncthreads();
+#pragma unroll
+    for (int w = 1; w < NWV; ++w) {
+      (*x)[0] += s_x[w][lane][0];
+      (*x)[1] += s_x[w][lane][1];
+    }
+  }
   return l;
 }
 // two channels of a joined row; place: it stands in its sequence
@@ -400,23 +414,13 @@ T2R_DEV void join_store(const BlkAttn& p, E* out, const float* x, float l, bool 
 // a workgroup per (head, sequence); 4.3 us, 3.3 of them an empty kernel's
 template <class E>
 __global__ __launch_bounds__(kBaThreads) void k_blk_step_join(BlkAttn p) {
-  __shared__ float s_x[kBaWaves][64][2];
-  const int h = blockIdx.x, b = blockIdx.y, wave = wave_index(), lane = threadIdx.x & 63;
+  const int h = blockIdx.x, b = blockIdx.y;
   const long long len = min((long long)p.g.lens[b], (long long)p.c.width << p.c.lbs);
   if (len <= p.chunk) return;                             // one part (or none): written already
   const int parts = (int)((len + p.chunk - 1) / p.chunk);
   float x[2];
-  const float l = join_parts<kBaWaves>(p, ((long long)b * p.H + h) * p.nsplit, parts, wave, &x);
-  s_x[wave][lane][0] = x[0];
-  s_x[wave][lane][1] = x[1];
-  __syncthreads();
-  if (wave > 0) return;
-#pragma unroll
-  for (int w = 1; w < kBaWaves; ++w) {
-    x[0] += s_x[w][lane][0];
-    x[1] += s_x[w][lane][1];
-  }
-  join_store<E>(p, (E*)p.out + (long long)b * p.out_ld + (long long)h * p.c.hd, x, l, true);
+  const float l = join_parts<kBaWaves>(p, ((long long)b * p.H + h) * p.nsplit, parts, &x);
+  if (wave_index() == 0) join_store<E>(p, (E*)p.out + (long long)b * p.out_ld + (long long)h * p.c.hd, x, l, true);
 }
 
 // ---------------------------------------------------------------- several rows a sequence
@@ -425,7 +429,7 @@ __global__ __launch_bounds__(kBaThreads) void k_blk_step_join(BlkAttn p) {
 //
 // k_blk_few: 32 columns. The four waves take every fourth 32 keys, each loading and converting its codes by itself: nothing
 // is shared but the columns, and no barrier stands in the loop. 8 rows of each of four sequences over 5003 .. 8100 positions,
-// 32 heads of 64: 17.6 us in parts of 512 keys, of which a part's beginning and end are half, and 4.9 for the join.
+// 32 heads of 64: 16 us in parts of 512 keys, of which a part's beginning and end are half, and 5.4 for the join.
 // k_blk_tile: 32 CT CG columns, CG groups of 32 CT for the waves; KG = 4 / CG waves of a group take the stage's 32 KG keys.
 // The workgroup loads a stage's codes together (a stage ahead), converts them once into LDS, in the MFMA operands' order,
 // two stages in turn with one barrier each. The conversion is as much vector work as the softmax of 32 columns (160
@@ -934,18 +938,19 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
   tile_end<E, HD, CT, CG>(p, t, kvh, blockIdx.y, k0 == 0 && kend == t.end, vref, m, l, o, ml, (float*)s_big);
 }
 
-// Joins the parts of a tile's columns: a wave a column
-template <class E>
+// Joins the parts of a tile's columns, NWV waves a column
+template <class E, int NWV>
 __global__ __launch_bounds__(kBaThreads) void k_blk_rows_join(BlkAttn p, int cols) {
   const int w_tile = blockIdx.x / p.c.Hk, kvh = blockIdx.x - w_tile * p.c.Hk;
   Tile t;
   if (!find_tile(p, cols, w_tile, &t) || t.end <= p.chunk) return;
-  const int cc = blockIdx.y * kBaWaves + wave_index();
+  const int cc = NWV > 1 ? (int)blockIdx.y : (int)blockIdx.y * kBaWaves + wave_index();
   if (cc >= t.rows * p.G) return;
   const int parts = (int)((t.end + p.chunk - 1) / p.chunk);
   float x[2];
-  const float l = join_parts<1>(p, ((long long)blockIdx.x * cols + cc) * p.nsplit, parts, 0, &x);
-  join_store<E>(p, (E*)p.out + col_at(t, p.G, p.c.hd, kvh, cc, p.out_ld), x, l, t.s.p0 + t.i0 + cc / p.G >= 0);
+  const float l = join_parts<NWV>(p, ((long long)blockIdx.x * cols + cc) * p.nsplit, parts, &x);
+  if (NWV == 1 || wave_index() == 0)
+    join_store<E>(p, (E*)p.out + col_at(t, p.G, p.c.hd, kvh, cc, p.out_ld), x, l, t.s.p0 + t.i0 + cc / p.G >= 0);
 }
 
 }  // namespace t2r

@@ -91,14 +91,18 @@ Cut rows_cut(int B, int rows, int H, int Hk, int hd, int block, int width) {
   // every sequence's last tile may be a part of one
   const long long tiles = rows / rt + (B < rows ? B : rows);
   c.tiles = (int)tiles;
-  const long long wgs = tiles * Hk;
   c.chunk = (int)cap;
   c.nsplit = 1;
-  // A part costs what a tile costs before and after its keys (7 us) and the join's launch (5 us); 64 keys of a tile take 1.3
+  // A part costs what a tile costs before and after its keys (7 us) and the join's launch (4 to 5 us); 64 keys of a tile take 1.3
   // us. So keys are cut only while workgroups leave half of the chip's places empty, and into parts of 512 at least: a
   // 1024-row prompt (256 workgroups) took 30 + 13 us in four parts and 31 whole, 8 rows at 8100 positions 200 us whole.
-  if (wgs <= 256) {
-    const long long want = 512 / wgs, ch = cdiv(cdiv(cap, want), 128) * 128;
+  // Few rows are one tile a sequence as a rule, three workgroups of which fit a CU: 8 rows of 16 sequences at 5000 .. 8100
+  // positions, 32 heads of 64, took 46 / 36 / 33 / 37 / 46 us in parts of 4096 / 2048 / 1280 / 1024 / 512 keys; of 4
+  // sequences 23 / 21 / 21 in parts of 2048 / 1024 / 512.
+  const bool few = c.cols == 32;
+  const long long wgs = (few ? B : tiles) * Hk, places = few ? 768 : 512;
+  if (wgs <= places / 2) {
+    const long long want = places / wgs, ch = cdiv(cdiv(cap, want), 128) * 128;
     c.chunk = (int)(ch < 512 ? 512 : ch);
     c.nsplit = (int)cdiv(cap, c.chunk);
   }
@@ -239,7 +243,8 @@ int t2r_attn_blk_prefill(const void* q, int dtype, int64_t q_ld, const int8_t* k
     } else {
       launch((k_blk_tile<E, 64, 2>), grid, block, 0, st, p);
     }
-    if (cut.nsplit > 1) launch(k_blk_rows_join<E>, dim3(cut.tiles * Hk, cut.cols / kBaWaves), block, 0, st, p, cut.cols);
+    if (cut.nsplit >= kJoinWide) launch((k_blk_rows_join<E, kBaWaves>), dim3(cut.tiles * Hk, cut.cols), block, 0, st, p, cut.cols);
+    else if (cut.nsplit > 1) launch((k_blk_rows_join<E, 1>), dim3(cut.tiles * Hk, cut.cols / kBaWaves), block, 0, st, p, cut.cols);
     return launched();
   });
 }
