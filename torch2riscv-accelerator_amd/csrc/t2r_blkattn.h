@@ -517,25 +517,33 @@ T2R_DEV void soft_max(v16f_t& s, float sk, int left, float& m, float& l, v16f_t*
     for (int i = 0; i < DT; ++i) o[i] *= al;
   }
 }
-// ... then the probabilities: that of key r, times its V block's share, as fp16 pieces ...
+// ... then the probabilities: those of keys r and r + 1, times their V block's share, as fp16 pieces, and their sum; ...
 template <int NP>
-T2R_DEV float soft_weight(float s, float sk, float add, v8h_t (*pf)[2], int r) {
-  const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s, sk, add));
-  const _Float16 h = (_Float16)w;
-  pf[0][r >> 3][r & 7] = h;
-  float minus = -1.0f;                                        // (kept from the compiler, which would take h out of fp16 to subtract it:
-  asm("" : "+s"(minus));                                      // so it is one mixed-precision step)
-  if (NP == 2) pf[NP - 1][r >> 3][r & 7] = (_Float16)__builtin_fmaf((float)h, minus, w);
-  return w;
+T2R_DEV float soft_weights(const v16f_t& s, float sk, float add, v8h_t (*pf)[2], int r) {
+  typedef float v2f_t __attribute__((ext_vector_type(2)));
+  const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sk, add)), w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], sk, add));
+  v2h_t h = __builtin_convertvector((v2f_t{w0, w1}), v2h_t);
+  // The low pieces in one mixed-precision step each, which reads the high ones where they are. (Both values are kept from the
+  // compiler, which would convert anew and take h out of fp16 to subtract it.)
+  float minus = -1.0f;
+  asm("" : "+v"(h));
+  asm("" : "+s"(minus));
+  pf[0][r >> 3][r & 7] = h[0];
+  pf[0][r >> 3][(r & 7) + 1] = h[1];
+  if (NP == 2) {
+    pf[NP - 1][r >> 3][r & 7] = (_Float16)__builtin_fmaf((float)h[0], minus, w0);
+    pf[NP - 1][r >> 3][(r & 7) + 1] = (_Float16)__builtin_fmaf((float)h[1], minus, w1);
+  }
+  return w0 + w1;
 }
 // ... of all 16, and their sum into l.
 template <int NP>
 T2R_DEV void soft_exp(const v16f_t& s, float sk, float lw, float iw, float m, float& l, v8h_t (*pf)[2]) {
   const float add = lw + kLift - (m == kNegInf ? 0.0f : m);
-  float ls[4] = {0, 0, 0, 0};
+  float ls[2] = {0, 0};
 #pragma unroll
-  for (int r = 0; r < 16; ++r) ls[r & 3] += soft_weight<NP>(s[r], sk, add, pf, r);
-  l = __builtin_fmaf((ls[0] + ls[1]) + (ls[2] + ls[3]), iw, l);
+  for (int r = 0; r < 16; r += 2) ls[r >> 1 & 1] += soft_weights<NP>(s, sk, add, pf, r);
+  l = __builtin_fmaf(ls[0] + ls[1], iw, l);
 }
 
 // The end of a tile: its waves' sums (wave's column group cg of 32 CT, key group kg of KG) are joined through LDS (so: KG x COLS
@@ -886,21 +894,21 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
       read_v(0);
       __builtin_amdgcn_sched_barrier(0);
       v8h_t pf[CT][NP][2];
-      float sk[CT], add[CT], ls[CT][2];
+      float sk[CT], add[CT], ls[CT];
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
         sk[ct] = score_scale(sq[ct], ks);
         soft_max<DT, edge.value>(s[ct], sk[ct], edge.value ? keys_left(at[ct], seg + ch * 16, seen) : 16, m[ct], l[ct], o[ct]);
         add[ct] = lw + kLift - (m[ct] == kNegInf ? 0.0f : m[ct]);
-        ls[ct][0] = ls[ct][1] = 0;
+        ls[ct] = 0;
       }
       // The probabilities of 8 keys, then their products; the other 8 keys' between those, the next loads between the last.
       auto weigh = [&](int r) {
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) ls[ct][r & 1] += soft_weight<NP>(s[ct][r], sk[ct], add[ct], pf[ct], r);
+        for (int ct = 0; ct < CT; ++ct) ls[ct] += soft_weights<NP>(s[ct], sk[ct], add[ct], pf[ct], r);
       };
 #pragma unroll
-      for (int r = 0; r < 8; ++r) weigh(r);
+      for (int r = 0; r < 8; r += 2) weigh(r);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int half = 0; half < 2; ++half)
@@ -912,7 +920,7 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
           if (half == 0) {
             if (g == 0) read_v(1);
 #pragma unroll
-            for (int r = 8 + g * 8 / (NP * DT); r < 8 + (g + 1) * 8 / (NP * DT); ++r) weigh(r);
+            for (int r = 4 + g * 4 / (NP * DT); r < 4 + (g + 1) * 4 / (NP * DT); ++r) weigh(2 * r);
           } else if (g == 0) {
             load_k(min(st + 2, last));
           } else if (g == 1) {
@@ -921,7 +929,7 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
           __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) l[ct] = __builtin_fmaf(ls[ct][0] + ls[ct][1], iw, l[ct]);
+      for (int ct = 0; ct < CT; ++ct) l[ct] = __builtin_fmaf(ls[ct], iw, l[ct]);
       __syncthreads();                                        // this buffer is read, the other one whole
     };
     const int plain = plain_steps(all_see, seg, n, STAGE, holes);
