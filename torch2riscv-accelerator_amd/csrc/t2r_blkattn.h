@@ -81,12 +81,12 @@ T2R_DEV float add_ror8(float x) {
   return x + fv((uint32_t)__builtin_amdgcn_update_dpp(0, (int)fb(x), 0x128, 0xF, 0xF, false));
 }
 
-// What a segment's keys need, 16 keys an entry: the (block, head) tile (-1: no block there, its keys are left out), the K
-// scale, and the V scale as a share of vref: its log2, which goes into the probabilities' exponent, and its inverse, which
+// What a segment's keys need, 16 keys an entry: where their codes begin in kc and in vc (0 where there is no block), how many
+// of them there are, the K scale, and the V scale as a share of vref: its log2, which goes into the probabilities' exponent, and its inverse, which
 // takes it out of their sum again. (A share below 2^-60 counts as that: its values are nothing beside vref's, the
 // probabilities' sum is right all the same.)
 struct BaSeg {
-  int tb[kBaSeg / 16];                        // (0 where there is none)
+  long long k_at[kBaSeg / 16], v_at[kBaSeg / 16];
   int seen[kBaSeg / 16];                      // 16, or fewer at the end, or none
   float ks[kBaSeg / 16], lw[kBaSeg / 16], iw[kBaSeg / 16];
   float red[kBaWaves];
@@ -94,7 +94,7 @@ struct BaSeg {
 };
 // The tables of the keys key0 .. key0 + n - 1, in whole steps of `step` keys, for the whole workgroup. In parts, so that what
 // a kernel has to load meanwhile is asked for between them: seg_table asks for this thread's table entry; seg_blocks puts the
-// tiles into LDS (a barrier: the codes can be asked for then); seg_scales the scales (a second one), and returns the larger
+// places into LDS (a barrier: the codes can be asked for then); seg_scales the scales (a second one), and returns the larger
 // of vref and the V scales among them; *holes: some of the n keys have no block.
 T2R_DEV int seg_table(const BlkCache& c, int b, long long key0, int n) {
   const int tid = threadIdx.x;
@@ -103,7 +103,10 @@ T2R_DEV int seg_table(const BlkCache& c, int b, long long key0, int n) {
 T2R_DEV void seg_blocks(BaSeg& sg, const BlkCache& c, int blk, int head, int n, int step) {
   const int tid = threadIdx.x, entries = (n + step - 1) / step * (step >> 4);
   if (tid < entries) {
-    sg.tb[tid] = max(blk, 0) * c.Hk + (blk < 0 ? 0 : head);
+    const long long tile = (long long)(max(blk, 0) * c.Hk + (blk < 0 ? 0 : head)) * c.tile_bytes();
+    const int in = (tid * 16) & (c.bs() - 1);             // (segments begin at whole blocks)
+    sg.k_at[tid] = tile + in * c.hd;
+    sg.v_at[tid] = tile + in;
     sg.seen[tid] = blk < 0 ? 0 : min(n - tid * 16, 16);
   }
   __syncthreads();
@@ -161,7 +164,7 @@ __global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_step(BlkAt
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_index(), col = lane & 15, c4 = lane >> 4;
   const int sets = (p.G + HW - 1) / HW;
   const int kvh = blockIdx.x / sets, h0 = (blockIdx.x - kvh * sets) * HW, b = blockIdx.y, split = blockIdx.z;
-  const int hd = p.c.hd, lbs = p.c.lbs, bmask = (1 << lbs) - 1;
+  const int hd = p.c.hd, lbs = p.c.lbs;
   const int nh = min(HW, p.G - h0);                       // heads of this workgroup
   const long long k0 = (long long)split * p.chunk;
   // everything that needs nothing loaded is asked for at once: the length, the table and q
@@ -183,13 +186,12 @@ __global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_step(BlkAt
       for (int i = tid; i < nh * hd; i += kBaThreads) out[i] = narrow<E>(0.0f);
     return;
   }
-  const int n = (int)min((long long)p.chunk, len - k0), steps = (n + 63) >> 6, tile = p.c.tile_bytes();
+  const int n = (int)min((long long)p.chunk, len - k0), steps = (n + 63) >> 6;
   const int mine = tid * 16 < n ? blk : -1;
   v4i_t kr[4][KU], vr[DT];
   // K rows: row m = 4 c' + r of the t-th 16 stands for key 16 c' + 4 t + r of the 64
   auto load_k = [&](int st) {
-    const int ch = st * 4 + (col >> 2);
-    const int8_t* base = p.c.kc + (long long)sg.tb[ch] * tile + (((ch * 16) & bmask) + (col & 3)) * hd;
+    const int8_t* base = p.c.kc + sg.k_at[st * 4 + (col >> 2)] + (col & 3) * hd;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -199,8 +201,7 @@ __global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_step(BlkAt
       }
   };
   auto load_v = [&](int st) {
-    const int ch = st * 4 + c4;
-    const int8_t* base = p.c.vc + (long long)sg.tb[ch] * tile + ((ch * 16) & bmask);
+    const int8_t* base = p.c.vc + sg.v_at[st * 4 + c4];
 #pragma unroll
     for (int i = 0; i < DT; ++i) vr[i] = *(const v4i_t*)(base + (min(i * 16 + col, hd - 1) << lbs));
   };
@@ -652,14 +653,14 @@ T2R_DEV int plain_steps(long long all_see, long long seg, int n, int step, bool 
 }
 
 template <class E, int HD>
-__global__ __launch_bounds__(kBaThreads, 2) void k_blk_few(BlkAttn p) {
+__global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_few(BlkAttn p) {
   constexpr int NP = Pieces<E>::kN, KU = HD / 32, DT = HD / 32;
   __shared__ BaSeg sg;
   using End = TileEnd<HD, 1, 1>;
   __shared__ typename End::Ml ml;
   __shared__ __align__(16) char s_o[End::kBytes];
   const int lane = threadIdx.x & 63, wave = wave_index(), col = lane & 31, c2 = lane >> 5;
-  const int hd = p.c.hd, lbs = p.c.lbs, bmask = (1 << lbs) - 1, G = p.G;
+  const int hd = p.c.hd, lbs = p.c.lbs, G = p.G;
   Tile t;
   int kvh;
   long long k0, kend;
@@ -670,7 +671,6 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_few(BlkAttn p) {
   q_load<E, KU>((const E*)p.q + col_at(t, G, hd, kvh, cc, p.q_ld), hd, x);
   v8h_t qf[KU][NP][2];
   const long long at = t.s.p0 + t.i0 + cc / G, all_see = t.s.p0 + t.i0 + 1;   // (keys below all_see are seen by every row)
-  const int tile = p.c.tile_bytes();
   // row 8 i + 4 c' + r of the 32 stands for key 16 c' + 4 i + r
   const int kc = (col >> 2) & 1, krow = 4 * (col >> 3) + (col & 3);
   float m = kNegInf, l = 0, vref = 0;
@@ -679,8 +679,7 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_few(BlkAttn p) {
   for (int i = 0; i < DT; ++i) o[0][i] = v16f_t{};
   v4i_t kr[KU], vr[DT];
   auto load_k = [&](int st) {
-    const int ch = st * 2 + kc;
-    const int8_t* base = p.c.kc + (long long)sg.tb[ch] * tile + (((ch * 16) & bmask) + krow) * hd;
+    const int8_t* base = p.c.kc + sg.k_at[st * 2 + kc] + krow * hd;
 #pragma unroll
     for (int u = 0; u < KU; ++u) {
       const int d = u * 32 + c2 * 16;
@@ -688,8 +687,7 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_few(BlkAttn p) {
     }
   };
   auto load_v = [&](int st) {
-    const int ch = st * 2 + c2;
-    const int8_t* base = p.c.vc + (long long)sg.tb[ch] * tile + ((ch * 16) & bmask);
+    const int8_t* base = p.c.vc + sg.v_at[st * 2 + c2];
 #pragma unroll
     for (int i = 0; i < DT; ++i) vr[i] = *(const v4i_t*)(base + (min(i * 32 + col, hd - 1) << lbs));
   };
@@ -770,10 +768,9 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
   __shared__ BaSeg sg;
   __shared__ typename End::Ml ml;
   __shared__ __align__(16) char s_big[kBufs > End::kBytes ? kBufs : End::kBytes];
-  v8h_t* bufs = (v8h_t*)s_big;
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_index(), col = lane & 31, c2 = lane >> 5;
   const int cg = wave % CG, kg = wave / CG;
-  const int hd = p.c.hd, lbs = p.c.lbs, bmask = (1 << lbs) - 1, G = p.G;
+  const int hd = p.c.hd, lbs = p.c.lbs, G = p.G;
   Tile t;
   int kvh;
   long long k0, kend;
@@ -795,38 +792,39 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
     for (int i = 0; i < DT; ++i) o[ct][i] = v16f_t{};
   }
   const long long all_see = t.s.p0 + t.i0 + 1;                // keys below this are seen by every row
-  const int tile = p.c.tile_bytes();
   v4i_t kr[PER], vr[PER];
-  // piece j of K: token j / (HD / 16), channels 16 (j % (HD / 16)); of V: channel j / (2 KG), tokens 16 (j % (2 KG))
+  // What this thread loads of a stage and where it puts it, in parts that no stage changes (an index worked out anew for each is
+  // vector work, which the kernel is bound by). Piece j = tid + 256 i of K: token j / (HD / 16), channels 16 (j % (HD / 16)); of
+  // V: channel j / (2 KG), tokens 16 (j % (2 KG)). The i'th piece lies KI tokens, VI channels after the first.
+  constexpr int KI = kBaThreads / (HD / 16), VI = kBaThreads / (2 * KG);
+  static_assert(PER == 1 || (KI % 32 == 0 && VI % 32 == 0), "whole fragments from piece to piece");
+  const int8_t *k_from, *v_from[PER];
+  int k_put, v_put;
+  {
+    const int key = tid / (HD / 16), dc = tid % (HD / 16), k16 = key & 15;
+    k_from = p.c.kc + (k16 * hd + (dc * 16 < hd ? dc * 16 : 0));
+    const int row = 8 * (k16 >> 2) + 4 * (key >> 4 & 1) + (k16 & 3);            // (the token's row of the 32)
+    k_put = (((key >> 5) * KU * 2 + (dc >> 1) * 2) * 64 + (((dc & 1) * 32 + row) ^ (dc & 7))) * 16;
+    const int ck = tid % (2 * KG), d = tid / (2 * KG);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) v_from[i] = p.c.vc + (min(d + i * VI, hd - 1) << lbs);
+    v_put = ((FR + (ck >> 1) * DT * 2 + (d >> 5) * 2) * 64 + (((ck & 1) * 32 + (d & 31)) ^ (2 * ck & 7))) * 16;
+  }
   auto load_k = [&](int st) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int j = tid + i * kBaThreads, key = st * STAGE + j / (HD / 16), d = j % (HD / 16) * 16;
-      kr[i] = *(const v4i_t*)(p.c.kc + (long long)sg.tb[key >> 4] * tile + ((key & bmask) * hd + (d < hd ? d : 0)));
-    }
+    for (int i = 0; i < PER; ++i) kr[i] = *(const v4i_t*)(k_from + sg.k_at[st * 2 * KG + (tid / (HD / 16) >> 4) + i * (KI / 16)]);
   };
   auto load_v = [&](int st) {
+    const long long at = sg.v_at[st * 2 * KG + tid % (2 * KG)];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int j = tid + i * kBaThreads, ch = st * 2 * KG + j % (2 * KG), d = j / (2 * KG);
-      vr[i] = *(const v4i_t*)(p.c.vc + (long long)sg.tb[ch] * tile + (((ch * 16) & bmask) + (min(d, hd - 1) << lbs)));
-    }
+    for (int i = 0; i < PER; ++i) vr[i] = *(const v4i_t*)(v_from[i] + at);
   };
-  // half of a loaded piece (K's PER, then V's) into its fragment
-  auto put_half = [&](v8h_t* buf, int h) {
+  // half of a loaded piece (K's PER, then V's) into its fragment of buffer 0 or 1
+  auto put_half = [&](int buf, int h) {
     const int i = h >> 1, half = h & 1;
-    int fr, slot;
-    if (i < PER) {
-      const int j = tid + i * kBaThreads, key = j / (HD / 16), dc = j % (HD / 16), k16 = key & 15;
-      fr = (key >> 5) * KU * 2 + (dc >> 1) * 2;
-      slot = ((dc & 1) * 32 + 8 * (k16 >> 2) + 4 * (key >> 4 & 1) + (k16 & 3)) ^ (dc & 7);   // (the token's row of the 32)
-      buf[(fr + half) * 64 + slot] = codes_h(kr[i][2 * half], kr[i][2 * half + 1]);
-    } else {
-      const int j = tid + (i - PER) * kBaThreads, ck = j % (2 * KG), d = j / (2 * KG);
-      fr = FR + (ck >> 1) * DT * 2 + (d >> 5) * 2;
-      slot = ((ck & 1) * 32 + (d & 31)) ^ (2 * ck & 7);
-      buf[(fr + half) * 64 + slot] = codes_h(vr[i - PER][2 * half], vr[i - PER][2 * half + 1]);
-    }
+    char* to = s_big + buf * (2 * FR * 1024);
+    if (i < PER) *(v8h_t*)(to + k_put + ((i * KI >> 5) * KU * 2 + half) * 1024) = codes_h(kr[i][2 * half], kr[i][2 * half + 1]);
+    else *(v8h_t*)(to + v_put + (((i - PER) * VI >> 5) * 2 + half) * 1024) = codes_h(vr[i - PER][2 * half], vr[i - PER][2 * half + 1]);
   };
   // a segment's blocks, and its first loads
   auto begin = [&](int n) {
@@ -850,12 +848,12 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
     vref = vmax;
     // (past the last stage loads repeat it, and nobody reads what is put of them)
 #pragma unroll
-    for (int h = 0; h < 4 * PER; ++h) put_half(bufs, h);
+    for (int h = 0; h < 4 * PER; ++h) put_half(0, h);
     load_k(min(1, last));
     load_v(min(1, last));
     __syncthreads();
     auto stage = [&](int st, auto edge) {
-      const v8h_t* buf = bufs + (st & 1) * 2 * FR * 64;
+      const v8h_t* buf = (const v8h_t*)s_big + (st & 1) * 2 * FR * 64;
       const int ch = ((st * STAGE + kg * 32) >> 4) + c2;
       v8h_t kf[KU][2], vf[DT][2];
       auto read_k = [&](int from, int to) {
@@ -873,7 +871,6 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
             v16f_t s[CT];
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) s[ct] = v16f_t{};
-      v8h_t* next = bufs + (~st & 1) * 2 * FR * 64;
       constexpr int GROUPS = KU * 2, EACH = 4 * PER / GROUPS;
       static_assert(EACH * GROUPS == 4 * PER, "the same number of pieces a group");
 #pragma unroll
@@ -884,7 +881,7 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
           for (int ct = 0; ct < CT; ++ct) s[ct] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[g >> 1][g & 1], qf[ct][g >> 1][q][g & 1], s[ct], 0, 0, 0);
         if (g == 0) read_k(KU / 2, KU);
 #pragma unroll
-        for (int h = 0; h < EACH; ++h) put_half(next, g * EACH + h);
+        for (int h = 0; h < EACH; ++h) put_half(~st & 1, g * EACH + h);
         __builtin_amdgcn_sched_barrier(0);
       }
       auto read_v = [&](int half) {
