@@ -518,33 +518,38 @@ T2R_DEV void soft_max(v16f_t& s, float sk, int left, float& m, float& l, v16f_t*
     for (int i = 0; i < DT; ++i) o[i] *= al;
   }
 }
-// ... then the probabilities: those of keys r and r + 1, times their V block's share, as fp16 pieces, and their sum; ...
+// ... then the probabilities: those of keys r .. r + 3, times their V block's share, as fp16 pieces, and their sum; ...
 template <int NP>
 T2R_DEV float soft_weights(const v16f_t& s, float sk, float add, v8h_t (*pf)[2], int r) {
   typedef float v2f_t __attribute__((ext_vector_type(2)));
-  const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sk, add)), w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], sk, add));
-  v2h_t h = __builtin_convertvector((v2f_t{w0, w1}), v2h_t);
-  // The low pieces in one mixed-precision step each, which reads the high ones where they are. (Both values are kept from the
-  // compiler, which would convert anew and take h out of fp16 to subtract it.)
-  float minus = -1.0f;
-  asm("" : "+v"(h));
-  asm("" : "+s"(minus));
-  pf[0][r >> 3][r & 7] = h[0];
-  pf[0][r >> 3][(r & 7) + 1] = h[1];
-  if (NP == 2) {
-    pf[NP - 1][r >> 3][r & 7] = (_Float16)__builtin_fmaf((float)h[0], minus, w0);
-    pf[NP - 1][r >> 3][(r & 7) + 1] = (_Float16)__builtin_fmaf((float)h[1], minus, w1);
+  float w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + i], sk, add));
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    v2h_t h = __builtin_convertvector((v2f_t{w[i], w[i + 1]}), v2h_t);
+    // The low pieces in one mixed-precision step each, which reads the high ones where they are. (Both values are kept from the
+    // compiler, which would convert anew and take h out of fp16 to subtract it.)
+    float minus = -1.0f;
+    asm("" : "+v"(h));
+    asm("" : "+s"(minus));
+    pf[0][r >> 3][(r & 7) + i] = h[0];
+    pf[0][r >> 3][(r & 7) + i + 1] = h[1];
+    if (NP == 2) {
+      pf[NP - 1][r >> 3][(r & 7) + i] = (_Float16)__builtin_fmaf((float)h[0], minus, w[i]);
+      pf[NP - 1][r >> 3][(r & 7) + i + 1] = (_Float16)__builtin_fmaf((float)h[1], minus, w[i + 1]);
+    }
   }
-  return w0 + w1;
+  return (w[0] + w[1]) + (w[2] + w[3]);
 }
 // ... of all 16, and their sum into l.
 template <int NP>
 T2R_DEV void soft_exp(const v16f_t& s, float sk, float lw, float iw, float m, float& l, v8h_t (*pf)[2]) {
   const float add = lw + kLift - (m == kNegInf ? 0.0f : m);
-  float ls[2] = {0, 0};
+  float ls = 0;
 #pragma unroll
-  for (int r = 0; r < 16; r += 2) ls[r >> 1 & 1] += soft_weights<NP>(s, sk, add, pf, r);
-  l = __builtin_fmaf(ls[0] + ls[1], iw, l);
+  for (int r = 0; r < 16; r += 4) ls += soft_weights<NP>(s, sk, add, pf, r);
+  l = __builtin_fmaf(ls, iw, l);
 }
 
 // The end of a tile: its waves' sums (wave's column group cg of 32 CT, key group kg of KG) are joined through LDS (so: KG x COLS
@@ -905,7 +910,7 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
         for (int ct = 0; ct < CT; ++ct) ls[ct] += soft_weights<NP>(s[ct], sk[ct], add[ct], pf[ct], r);
       };
 #pragma unroll
-      for (int r = 0; r < 8; r += 2) weigh(r);
+      for (int r = 0; r < 8; r += 4) weigh(r);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int half = 0; half < 2; ++half)
@@ -917,7 +922,7 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
           if (half == 0) {
             if (g == 0) read_v(1);
 #pragma unroll
-            for (int r = 4 + g * 4 / (NP * DT); r < 4 + (g + 1) * 4 / (NP * DT); ++r) weigh(2 * r);
+            for (int r = 2 + g * 2 / (NP * DT); r < 2 + (g + 1) * 2 / (NP * DT); ++r) weigh(4 * r);
           } else if (g == 0) {
             load_k(min(st + 2, last));
           } else if (g == 1) {
