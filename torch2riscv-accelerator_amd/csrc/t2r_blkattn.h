@@ -431,15 +431,17 @@ __global__ __launch_bounds__(kBaThreads) void k_blk_step_join(BlkAttn p) {
 // k_blk_few: 32 columns. The four waves take every fourth 32 keys, each loading and converting its codes by itself: nothing
 // is shared but the columns, and no barrier stands in the loop. 8 rows of each of four sequences over 5003 .. 8100 positions,
 // 32 heads of 64: 16 us in parts of 512 keys, of which a part's beginning and end are half, and 5.4 for the join.
-// k_blk_tile: 32 CT CG columns, CG groups of 32 CT for the waves; KG = 4 / CG waves of a group take the stage's 32 KG keys.
-// The workgroup loads a stage's codes together (a stage ahead), converts them once into LDS, in the MFMA operands' order,
-// two stages in turn with one barrier each. The conversion is as much vector work as the softmax of 32 columns (160
-// instructions of 32 keys at head dim 128 against 180), so CG waves share it. Measured: one prompt of 2032 rows, 16 heads of 128
-// in fp32, 54.6 us (310 TFLOP/s of the formula's, twice that of fp16 products, q and p being two pieces); seven prompts and
-// turns in bf16, 32 heads of 64, 76 us (475 TFLOP/s). The last tiles of a long prompt set the time, 32 stages of 1.25 us after
-// 7 us before and after; in a wave the products of a stage (2 x 512 cycles at head dim 128 in fp32) and its 900 cycles of
-// softmax, conversions and LDS traffic add up, and the second workgroup of the CU hides little of the sum. More waves a
-// workgroup, a second stage in flight in registers and tiles cut along their keys all came out slower.
+// k_blk_tile: 64 CT columns, two groups of 32 CT for the waves; the two waves of a group take the stage's two times 32 keys. The
+// workgroup loads a stage's codes together (a stage ahead), converts them once into LDS, in the MFMA operands' order, two
+// stages in turn with one barrier each. The conversion is as much vector work as the softmax of 32 columns (80 instructions of
+// 32 keys at head dim 128 where two waves share it, against 100), so the groups share it.
+// Bound by issue: a product takes 32 cycles of its unit and a vector instruction 4, five where a SIMD has one wave, and beyond
+// three a product they add up. At head dim 128 in fp32 a wave has 32 products and 194 other vector instructions a stage, in
+// bf16 at 64 16 and 180. One prompt of 2032 rows, 16 heads of 128 in fp32: 53 us (318 TFLOP/s of the formula's, twice that of
+// fp16 products, q and p being two pieces), 1.17 us a stage where one workgroup is on a CU, 1.03 where two are, so each CU's
+// 33 stages take about as long however tiles are cut or paired; 7 us a tile lie before and after them. Seven prompts and turns
+// in bf16, 32 heads of 64: 74 us (488 TFLOP/s). Slower, all measured: eight waves a workgroup, a second stage in flight in
+// registers, tiles cut along their keys; four groups of 32 columns at head dim 128 gain 0 .. 10% past 8000 rows and lose before.
 struct Tile {
   Seq s;
   int t, i0, rows;          // tile t of sequence s: its rows i0 .. i0 + rows - 1
@@ -760,8 +762,7 @@ __global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_few(BlkAtt
 // [kg][u][half], V's [kg][i][half]. The lane's slot is turned by the fragment's place, so that the loading threads, which
 // hold neighbouring 16-byte pieces of a token or channel, write to different banks.
 //
-// The waves of the two workgroups that share a SIMD drift apart, so that one's products run beside the other's softmax. What a
-// wave has to wait for is kept off its own path: a stage's codes are loaded a stage ahead, its V fragments are read from LDS
+// What a wave has to wait for is kept off its path: a stage's codes are loaded a stage ahead, its V fragments are read from LDS
 // before the softmax, and two buffers leave one barrier a stage.
 template <class E, int HD, int CT>
 __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {

@@ -84,8 +84,8 @@ Cut rows_cut(int B, int rows, int H, int Hk, int hd, int block, int width) {
   Cut c;
   // Few rows: one tile of 32 columns a sequence. Else 64; 128, which a conversion of codes then serves, at head dims whose sums
   // leave a wave registers for two times 32, once 64 would be more than the chip has places for twice (1024). 32 heads of 64,
-  // one prompt of 512 / 2032 / 4064 rows, us: fp32 13.6 / 55.2 / 186 in 64 columns and 18.8 / 56.0 / 174 in 128, bf16 11.6 /
-  // 40.8 / 130 and 15.0 / 40.2 / 116.
+  // one prompt of 512 / 2032 / 4064 rows, us: fp32 13.1 / 51.4 / 175 in 64 columns and 18.0 / 52.5 / 156 in 128, bf16 11.2 /
+  // 40.1 / 122 and 15.1 / 40.0 / 111.
   c.cols = (long long)rows * G <= 32LL * B ? 32 : hd <= 64 && (long long)rows * H > 64 * 1024 ? 128 : 64;
   const int rt = c.cols / G;
   // every sequence's last tile may be a part of one
