@@ -142,6 +142,28 @@ def test_append_borders(env):
         c.same()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("top", [127.0, 1.875, 1.9765625, 0.0234375, 127 * 2.0 ** -12])
+def test_append_halves_of_16_bit_rows(env, dtype, top):
+    """Ties (scales that are powers of two) and values a rounding beside them (half of the largest value, 63.5 steps but for the
+    scale's rounding), with zeros, infinities and NaN among them, into empty and partly filled blocks."""
+    torch, ops = env
+    rng = np.random.default_rng(23)
+    Hk, hd, block, rows = 2, 64, 32, 50
+    x = rng.choice(np.r_[np.arange(-63, 63) + 0.5, -63.5, 63.5, 127, -127, 0, 21.5, 42.25, 31.75], (rows, 2, Hk, hd)) * (top / 127)
+    x[0] = top
+    x, t = rounded(torch, x.reshape(rows, -1), dtype)
+    c = Both(torch, ops, rng, [rows + 7], Hk, hd, block).send()
+    n = Hk * hd
+    for r0, r1, at in ((0, 7, 7), (0, rows, rows + 7)):
+        if r1 == rows:
+            t[9, 3], t[11, n + 5], t[12, 8] = np.inf, -np.inf, np.nan
+            x = t.double().cpu().numpy()
+        c.host.append(x[r0:r1, :n].astype(F), x[r0:r1, n:].astype(F), c.table, [0, r1 - r0], [at])
+        ops.kv_append_block(t[r0:r1, :n], t[r0:r1, n:], *c.dev, i32(torch, [0, r1 - r0]), i32(torch, [at]))
+        c.same()
+
+
 def test_append_places_without_a_block(env):
     """Rows below position 0, past the table, and at table entries outside the pool are dropped; slots behind the rows and
     other blocks keep what they hold; rows of no sequence are left out."""
