@@ -142,13 +142,8 @@ __global__ __launch_bounds__(kLpThreads, 4) void k_lp_part(LpArgs p) {
     const long long i0 = start_of(sp);
     if (sp >= p.spans || i0 >= V) return;
     if (i0 >= 0 && i0 + kLpSpan <= V) {
-      if (off == 0 && (uintptr_t)x % 16) {
 #pragma unroll
-        for (int i = 0; i < NL; ++i) w[i] = ((const Vec*)(x + i0 + i * kLpThreads * PER))[tid].v;
-      } else {
-#pragma unroll
-        for (int i = 0; i < NL; ++i) w[i] = ((const v4i_t*)(x + i0 + i * kLpThreads * PER))[tid];
-      }
+      for (int i = 0; i < NL; ++i) w[i] = ((const v4i_t*)(x + i0 + i * kLpThreads * PER))[tid];
     } else if (V >= PER) {
 #pragma unroll
       for (int i = 0; i < NL; ++i) w[i] = ((const Vec*)(x + min(max(i0 + (i * kLpThreads + tid) * PER, 0LL), (long long)V - PER)))->v;
