@@ -138,6 +138,9 @@ __global__ __launch_bounds__(kLpThreads, 4) void k_lp_part(LpArgs p) {
   v4i_t w[NL];
   const int off = V >= kLpSpan ? (int)((uintptr_t)x % 16 / sizeof(E)) : 0;
   auto start_of = [&](int sp) { return ((long long)part * p.spans + sp) * kLpSpan - off; };
+  // the places of a span at i0 where the row begins, and where its last PER values do (before the span where few are left)
+  auto first_of = [&](long long i0) { return (int)max(-i0, 0LL); };
+  auto last_of = [&](long long i0) { return (int)min(V - PER - i0, (long long)kLpSpan); };
   auto fetch = [&](int sp) {
     const long long i0 = start_of(sp);
     if (sp >= p.spans || i0 >= V) return;
@@ -145,8 +148,9 @@ __global__ __launch_bounds__(kLpThreads, 4) void k_lp_part(LpArgs p) {
 #pragma unroll
       for (int i = 0; i < NL; ++i) w[i] = ((const v4i_t*)(x + i0 + i * kLpThreads * PER))[tid];
     } else if (V >= PER) {
+      const int first = first_of(i0), last = last_of(i0);
 #pragma unroll
-      for (int i = 0; i < NL; ++i) w[i] = ((const Vec*)(x + min(max(i0 + (i * kLpThreads + tid) * PER, 0LL), (long long)V - PER)))->v;
+      for (int i = 0; i < NL; ++i) w[i] = ((const Vec*)(x + i0 + min(max((i * kLpThreads + tid) * PER, first), last)))->v;
     } else {
       // a row of fewer values than a load takes: thread 0's first load, by hand, its values at the end
       for (int i = 0; i < NL; ++i) w[i] = v4i_t{0, 0, 0, 0};
@@ -218,11 +222,11 @@ __global__ __launch_bounds__(kLpThreads, 4) void k_lp_part(LpArgs p) {
     const bool whole = i0 >= 0 && i0 + kLpSpan <= V;
     uint32_t mine = ~0u;                                               // the values of its loads that are this thread's
     if (!whole) {
+      const int first = first_of(i0), last = last_of(i0);
       mine = 0;
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
-        const int at = (i * kLpThreads + tid) * PER;
-        const int before = (int)min(max(-i0 - at, 0LL), (long long)PER), past = (int)min(max(i0 + at - (V - PER), 0LL), (long long)PER);
+        const int at = (i * kLpThreads + tid) * PER, before = min(max(first - at, 0), PER), past = min(max(at - last, 0), PER);
         mine |= ((1u << PER) - 1) >> before >> past << past << (i * PER);
       }
     }
