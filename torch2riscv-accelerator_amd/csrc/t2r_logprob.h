@@ -6,7 +6,7 @@
 //
 // fp32 logits are bound by memory (1024 rows of 151936, top 20: 116 us, 5.4 TB/s), 16-bit ones by the vector units: six
 // instructions a value, one of them an exponential that counts four times, and what a span needs besides. 2032 rows of 49155:
-// 52 us with the top 5 (3.8 TB/s), 43 without; of 128256: 112 us with the top 20 (4.6), 98 without. Few rows: 16 of 128256
+// 51 us with the top 5 (3.9 TB/s), 42 without; of 128256: 110 us with the top 20 (4.7), 101 without. Few rows: 16 of 128256
 // 7.0 us and 6.6 for the join, an empty kernel taking 3.3.
 #pragma once
 #include "t2r_block.h"
