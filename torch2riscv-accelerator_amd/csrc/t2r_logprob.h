@@ -209,8 +209,8 @@ __global__ __launch_bounds__(kLpThreads, 4) void k_lp_part(LpArgs p) {
       if (k != 0 && r < top) next[r] = k;
     }
     now ^= 1;
-    if (tid == 0) s.keys = 0;
     __syncthreads();
+    if (tid == 0) s.keys = 0;                                          // (every thread has read it; the next span's barrier follows)
     bound = max(bound, (uint32_t)(s.best[now][top - 1] >> 32));
   };
   int noted = 0;                                                       // loads of earlier spans
