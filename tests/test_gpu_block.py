@@ -456,7 +456,8 @@ def test_offsets_past_32_bits(env):
 # ------------------------------------------------------------------ log probabilities
 def lp_check(torch, x, got, tokens, top, spans):
     """Sums of e^(x - m) over 32 values a thread and span, then a tree: (32 spans + 16) 2^-24 relative, the exponentials
-    2^-22 each and |x - m| 2^-23 of their argument, weighted by them: D = sum p |x - m|; m, ln l and x_t - lse are rounded."""
+    2^-22 each and |x - m| 2^-23 of their argument, weighted by them: D = sum p |x - m|, at most the entropy where m is the
+    maximum and 4 more where it is a thread's (rows past a span: ln V > 9); m, ln l and x_t - lse are rounded."""
     lp, ent, ids, val = (None if t is None else t.cpu().numpy() for t in got)
     wl, we, wi, wv = logprobs(x, tokens, top)
     assert np.array_equal(ids, wi)
