@@ -40,7 +40,7 @@ struct BlkAttn {
   int H, G;                 // heads, heads of a KV head
   float a;                  // softmax scale times log2(e)
   int order;                // find_piece's, of the tiles
-  int chunk, nsplit;        // keys of a workgroup (a multiple of its waves' step, at most kBaSeg when nsplit > 1)
+  int chunk, nsplit;        // keys of a workgroup (a multiple of 128 where there are several; the step form: at most kBaSeg)
   float* ws_o;              // parts of long rows: [row's column, split, hd] sums, and [.., 2] maxima and weights
   float* ws_ml;
 };
