@@ -410,6 +410,26 @@ def test_many_rows(env, H, Hk, hd, block, news, lens, dtype):
     check(torch, got, want, bound, dtype)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("H,Hk,hd,block,news,lens,width", [
+    (32, 8, 64, 64, [548], [4500], 128),
+    (16, 8, 128, 32, [300, 0, 251], [3300, 40, 2900], 256),
+    (32, 8, 48, 128, [270, 33], [3000, 33], 32),                             # (one of them within the first part)
+])
+def test_turns_late_in_long_caches(env, H, Hk, hd, block, news, lens, width, dtype):
+    """Some hundred rows, whose tiles' keys are cut into a few long parts. A few rows are compared."""
+    torch, ops = env
+    rng = np.random.default_rng(24)
+    c = Both(torch, ops, rng, lens, Hk, hd, block, width=width).fill(rng, spread=1.5).send()
+    starts = np.concatenate([[0], np.cumsum(news)])
+    rows = int(starts[-1])
+    x, t = rounded(torch, rng.standard_normal((rows, H * hd)), dtype)
+    got = ops.attention_block_prefill(t, *c.dev, i32(torch, starts), c.lens_d, H)
+    only = sorted({0, 15, 16, news[0] - 1, min(news[0], rows - 1), rows - 2, rows - 1})
+    want, bound = attention(c.host, x, c.table, starts, lens, H, 1 / math.sqrt(hd), 0 if dtype == "f32" else 2.0 ** -11, only=only)
+    check(torch, got, want, bound, dtype)
+
+
 def test_many_sequences_with_few_rows(env):
     """More sequences than a wave has lanes, most of them without rows."""
     torch, ops = env

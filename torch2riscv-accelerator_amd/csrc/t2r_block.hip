@@ -99,11 +99,17 @@ Cut rows_cut(int B, int rows, int H, int Hk, int hd, int block, int width) {
   // Few rows are one tile a sequence as a rule, three workgroups of which fit a CU: 8 rows of 16 sequences at 5000 .. 8100
   // positions, 32 heads of 64, took 46 / 36 / 33 / 37 / 46 us in parts of 4096 / 2048 / 1280 / 1024 / 512 keys; of 4
   // sequences 23 / 21 / 21 in parts of 2048 / 1024 / 512.
+  // Turns of a few hundred rows late in long caches (tables past 2048 positions) gain from a second workgroup on every CU, in
+  // parts of 1536 at least: 548 rows at 7127 positions, 32 heads of 64 in bf16 (280 workgroups), took 103 us whole and 86 / 81 /
+  // 80 / 78 / 83 in parts of 4096 / 2688 / 2048 / 1536 / 1024; 1200 at 8000, 16 heads of 128 (304), 160 and 148 / 141 / 138 / 141 /
+  // 152; but 900 rows (456) 99 whole and 111 to 123 in parts.
   const bool few = c.cols == 32;
-  const long long wgs = (few ? B : tiles) * Hk, places = few ? 768 : 512;
-  if (wgs <= places / 2) {
-    const long long want = places / wgs, ch = cdiv(cdiv(cap, want), 128) * 128;
-    c.chunk = (int)(ch < 512 ? 512 : ch);
+  const long long wgs = (few ? B : tiles) * Hk;
+  const bool turns = !few && wgs > 128 && cap > 2048;
+  const long long parts = few ? 768 : turns ? 1024 : 512, least = turns ? 1536 : 512;
+  if (wgs <= (turns ? 432 : parts / 2)) {
+    const long long want = parts / wgs, ch = cdiv(cdiv(cap, want), 128) * 128;
+    c.chunk = (int)(ch < least ? least : ch);
     c.nsplit = (int)cdiv(cap, c.chunk);
   }
   return c;
