@@ -82,7 +82,7 @@ def test_logprobs_refuses():
     ok = dict(x=P, dtype=0, ld=100, tokens=P, rows=2, V=100, top=3, lp=P, ent=P, ids=P, val=P, ws=P, ws_bytes=1 << 20)
     for kw, code in ((dict(x=None), abi.T2R_EINVAL), (dict(tokens=None), abi.T2R_EINVAL), (dict(ids=None), abi.T2R_EINVAL),
                      (dict(val=None), abi.T2R_EINVAL), (dict(dtype=-1), abi.T2R_EINVAL), (dict(x=ODD), abi.T2R_EINVAL),
-                     (dict(rows=0), abi.T2R_ESHAPE), (dict(rows=1 << 24), abi.T2R_ESHAPE), (dict(V=0), abi.T2R_ESHAPE), (dict(ld=99), abi.T2R_ESHAPE),
+                     (dict(rows=0), abi.T2R_ESHAPE), (dict(rows=1 << 24), abi.T2R_ESHAPE), (dict(V=0), abi.T2R_ESHAPE), (dict(V=2 ** 31 - 1, ld=2 ** 31), abi.T2R_ESHAPE), (dict(ld=99), abi.T2R_ESHAPE),
                      (dict(top=-1), abi.T2R_ERANGE), (dict(top=33), abi.T2R_ERANGE), (dict(V=2, top=3), abi.T2R_ERANGE),
                      (dict(V=20000, ld=20000, ws=None), abi.T2R_ENOMEM), (dict(V=20000, ld=20000, ws_bytes=10), abi.T2R_ENOMEM)):
         assert lib.t2r_logprobs(*{**ok, **kw}.values(), None) == code, kw
