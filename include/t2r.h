@@ -208,9 +208,9 @@ int t2r_attn_blk_prefill(const void* q, int dtype, int64_t q_ld, const int8_t* k
                          int64_t out_ld, void* workspace, int64_t workspace_bytes, void* stream);
 /* Log probabilities of logits rows [rows, V], ld elements apart: logprob[r] = log softmax(x[r])[tokens[r]]
  * (NaN for a token outside [0, V)), entropy[r] = -sum p ln p, and the `top` (<= 32, <= V) largest values in descending order,
- * the lower index first on ties and a NaN before everything: top_ids, top_logprob [rows, top]. V < 2^31 - 2^14. logprob (with tokens) and
- * entropy may be NULL. Values of -inf have probability 0; a row of nothing else gives -inf and entropy 0, a row with a
- * NaN or +inf gives NaN. Workspace (device, 16-byte aligned): t2r_logprobs_workspace_bytes, 0 may be NULL; one call's
+ * the lower index first on ties and a NaN before everything: top_ids, top_logprob [rows, top]. V < 2^31 - 2^14. logprob (with
+ * tokens) and entropy may be NULL. Values of -inf have probability 0; a row of nothing else gives -inf and entropy 0, a row
+ * with a NaN or +inf gives NaN. Workspace (device, 16-byte aligned): t2r_logprobs_workspace_bytes, 0 may be NULL; one call's
  * scratch. */
 int64_t t2r_logprobs_workspace_bytes(int rows, int V, int top);
 int t2r_logprobs(const void* logits, int dtype, int64_t ld, const int32_t* tokens, int rows, int V, int top,
