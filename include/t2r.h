@@ -195,8 +195,8 @@ int t2r_kv_read_blk(const int8_t* kc, const int8_t* vc, const float* ks, const f
  * spans less than 2^27 positions.
  * _prefill: ragged rows, each sees the positions up to its own. A row below position 0 (lens[b] less than the sequence's
  * rows) has no place in its sequence and gives NaN.
- * Workspace (device, 16-byte aligned): t2r_attn_blk_workspace_bytes with rows = 0 for _decode; 0 bytes may be NULL. It is
- * one call's scratch: calls that may overlap need one each. */
+ * Workspace (device, 16-byte aligned): t2r_attn_blk_workspace_bytes with rows = 0 for _decode (-1 for sizes that the call
+ * refuses); 0 bytes may be NULL. It is one call's scratch: calls that may overlap need one each. */
 int64_t t2r_attn_blk_workspace_bytes(int B, int rows, int H, int Hk, int hd, int block, int width, int dtype);
 int t2r_attn_blk_decode(const void* q, int dtype, int64_t q_ld, const int8_t* kc, const int8_t* vc, const float* ks,
                         const float* vs, int n_blocks, int block, int Hk, int hd, const int32_t* table, int width,
@@ -210,8 +210,8 @@ int t2r_attn_blk_prefill(const void* q, int dtype, int64_t q_ld, const int8_t* k
  * (NaN for a token outside [0, V)), entropy[r] = -sum p ln p, and the `top` (<= 32, <= V) largest values in descending order,
  * the lower index first on ties and a NaN before everything: top_ids, top_logprob [rows, top]. V < 2^31 - 2^14. logprob (with
  * tokens) and entropy may be NULL. Values of -inf have probability 0; a row of nothing else gives -inf and entropy 0, a row
- * with a NaN or +inf gives NaN. Workspace (device, 16-byte aligned): t2r_logprobs_workspace_bytes, 0 may be NULL; one call's
- * scratch. */
+ * with a NaN or +inf gives NaN. Workspace (device, 16-byte aligned): t2r_logprobs_workspace_bytes (-1 for sizes that the call
+ * refuses), 0 may be NULL; one call's scratch. */
 int64_t t2r_logprobs_workspace_bytes(int rows, int V, int top);
 int t2r_logprobs(const void* logits, int dtype, int64_t ld, const int32_t* tokens, int rows, int V, int top,
                  float* logprob, float* entropy, int32_t* top_ids, float* top_logprob, void* workspace,

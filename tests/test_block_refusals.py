@@ -70,6 +70,22 @@ def test_attention_refuses_its_own():
     assert lib.t2r_attn_blk_workspace_bytes(1, 0, 5, 2, 64, 64, 128, 0) == -1
 
 
+@pytest.mark.parametrize("sizes", [
+    (384, 384, 1, 1, 64, 1 << 30, 1 << 30, 0),                             # (a cut of 2^32 keys is 0 in 32 bits)
+    (1, 0, 4, 2, 64, 48, 100, 0), (1, 0, 4, 2, 72, 64, 100, 0), (1, 0, 4, 2, 144, 64, 100, 0), (1, 0, 4, 2, 64, 128, 1 << 24, 0),
+    (1, 0, 4, 2, 64, 64, 1 << 22, 0), (65536, 0, 4, 2, 64, 64, 100, 0), (1, 0, 1 << 17, 1 << 16, 64, 64, 100, 0),
+    (1, 1 << 24, 4, 2, 64, 64, 100, 0), (1, -1, 4, 2, 64, 64, 100, 0), (1, 1 << 23, 128, 4, 128, 64, 64, 0),
+    (2 ** 31 - 1, 0, 2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1, 0), (1, 0, 4, 2, 64, 64, 100, 3)])
+def test_attention_workspace_of_sizes_that_the_calls_refuse(sizes):
+    assert abi.load().t2r_attn_blk_workspace_bytes(*sizes) == -1
+
+
+@pytest.mark.parametrize("sizes", [(1000, 20000, 33), (1, 2 ** 31 - 1, 5), (1, 2, 3), (1 << 24, 100, 1), (1, 20000, -1),
+                                   (2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1)])
+def test_logprobs_workspace_of_sizes_that_the_call_refuses(sizes):
+    assert abi.load().t2r_logprobs_workspace_bytes(*sizes) == -1
+
+
 def test_read_refuses():
     lib = abi.load()
     ok = dict(kc=P, vc=P, ks=P, vs=P, n=4, block=64, Hk=2, hd=64, table=P, width=2, starts=P, lens=P, B=1, rows=1, dtype=0, k=P, v=P)

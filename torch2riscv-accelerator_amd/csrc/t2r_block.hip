@@ -32,14 +32,17 @@ int by_type(int dtype, F f) {
   }
 }
 
+// the cache's sizes but for the pool's
+bool cache_sizes_ok(int block, int Hk, int hd, int width) {
+  if (block != 16 && block != 32 && block != 64 && block != 128) return false;
+  return hd > 0 && hd <= 128 && hd % 16 == 0 && Hk > 0 && Hk <= 65535 && width > 0 && (long long)width * block <= INT32_MAX;
+}
 // the cache's description, checked; T2R_OK or a code
 int cache_args(const int8_t* kc, const int8_t* vc, const float* ks, const float* vs, int n_blocks, int block, int Hk,
                int hd, const int32_t* table, int width, BlkCache* c) {
   if (!kc || !vc || !ks || !vs || !table) return T2R_EINVAL;
   if (misaligned(kc, 16) || misaligned(vc, 16) || misaligned(ks, 4) || misaligned(vs, 4) || misaligned(table, 4)) return T2R_EINVAL;
-  if (block != 16 && block != 32 && block != 64 && block != 128) return T2R_ESHAPE;
-  if (hd <= 0 || hd > 128 || hd % 16 || Hk <= 0 || Hk > 65535 || n_blocks <= 0 || width <= 0) return T2R_ESHAPE;
-  if ((long long)n_blocks * Hk > INT32_MAX || (long long)width * block > INT32_MAX) return T2R_ESHAPE;
+  if (!cache_sizes_ok(block, Hk, hd, width) || n_blocks <= 0 || (long long)n_blocks * Hk > INT32_MAX) return T2R_ESHAPE;
   c->kc = (int8_t*)kc; c->vc = (int8_t*)vc; c->ks = (float*)ks; c->vs = (float*)vs; c->table = table;
   c->n_blocks = n_blocks; c->Hk = Hk; c->hd = hd; c->lbs = __builtin_ctz((unsigned)block); c->width = width;
   return T2R_OK;
@@ -116,6 +119,18 @@ Cut rows_cut(int B, int rows, int H, int Hk, int hd, int block, int width) {
 }
 
 bool attn_shape_ok(int H, int Hk) { return Hk > 0 && H > 0 && H % Hk == 0 && H / Hk <= 32; }
+// The two forms' sizes, of the calls and of the workspace query alike (the cuts are worked out for these only); the cut, or
+// false where a launch cannot hold it
+bool step_sizes(int B, int H, int Hk, int hd, int block, int width, int dtype, Cut* c) {
+  if (!attn_shape_ok(H, Hk) || B <= 0 || B > 65535 || H > 65535) return false;
+  *c = step_cut(B, H, Hk, hd, block, width, dtype);
+  return c->nsplit <= 65535;
+}
+bool rows_sizes(int B, int rows, int H, int Hk, int hd, int block, int width, Cut* c) {
+  if (!attn_shape_ok(H, Hk) || B <= 0 || rows <= 0 || rows >= kMaxRows) return false;
+  *c = rows_cut(B, rows, H, Hk, hd, block, width);
+  return c->nsplit <= 65535 && (long long)c->tiles * Hk <= kMaxGroups;
+}
 long long part_bytes(long long parts, int hd) { return parts * 4 * (hd + 2); }
 long long step_ws(const Cut& c, int B, int H, int hd) { return c.nsplit > 1 ? part_bytes((long long)B * H * c.nsplit, hd) : 0; }
 long long rows_ws(const Cut& c, int Hk, int hd) {
@@ -129,6 +144,12 @@ Cut lp_cut(int rows, int V) {             // chunk: spans a part takes; nsplit: 
   const long long per = cdiv(spans, want < spans ? want : spans);
   return Cut{(int)per, (int)cdiv(spans, per), 0, 0};
 }
+bool lp_sizes(int rows, int V, Cut* c) {
+  if (rows <= 0 || V <= 0 || V > INT32_MAX - 2 * kLpSpan) return false;
+  *c = lp_cut(rows, V);
+  return (long long)rows * c->nsplit <= kMaxGroups;
+}
+long long lp_ws(const Cut& c, int rows, int top) { return c.nsplit > 1 ? (long long)rows * c.nsplit * (16 + 8LL * top) : 0; }
 
 }  // namespace
 
@@ -178,8 +199,10 @@ int t2r_kv_read_blk(const int8_t* kc, const int8_t* vc, const float* ks, const f
 }
 
 int64_t t2r_attn_blk_workspace_bytes(int B, int rows, int H, int Hk, int hd, int block, int width, int dtype) {
-  if (B <= 0 || rows < 0 || !attn_shape_ok(H, Hk) || hd <= 0 || block <= 0 || width <= 0 || !dtype_ok(dtype)) return -1;
-  return rows == 0 ? step_ws(step_cut(B, H, Hk, hd, block, width, dtype), B, H, hd) : rows_ws(rows_cut(B, rows, H, Hk, hd, block, width), Hk, hd);
+  if (!cache_sizes_ok(block, Hk, hd, width) || !dtype_ok(dtype)) return -1;
+  Cut c;
+  if (rows == 0) return step_sizes(B, H, Hk, hd, block, width, dtype, &c) ? step_ws(c, B, H, hd) : -1;
+  return rows_sizes(B, rows, H, Hk, hd, block, width, &c) ? rows_ws(c, Hk, hd) : -1;
 }
 
 int t2r_attn_blk_decode(const void* q, int dtype, int64_t q_ld, const int8_t* kc, const int8_t* vc, const float* ks,
@@ -191,9 +214,8 @@ int t2r_attn_blk_decode(const void* q, int dtype, int64_t q_ld, const int8_t* kc
   BlkAttn p;
   std::memset(&p, 0, sizeof(p));
   if (int rc = cache_args(kc, vc, ks, vs, n_blocks, block, Hk, hd, table, width, &p.c)) return rc;
-  if (!attn_shape_ok(H, Hk) || B <= 0 || B > 65535 || H > 65535 || q_ld < (int64_t)H * hd || out_ld < (int64_t)H * hd) return T2R_ESHAPE;
-  const Cut cut = step_cut(B, H, Hk, hd, block, width, dtype);
-  if (cut.nsplit > 65535) return T2R_ESHAPE;
+  Cut cut;
+  if (!step_sizes(B, H, Hk, hd, block, width, dtype, &cut) || q_ld < (int64_t)H * hd || out_ld < (int64_t)H * hd) return T2R_ESHAPE;
   const long long need = step_ws(cut, B, H, hd);
   if (need > 0 && (!workspace || workspace_bytes < need || misaligned(workspace, 16))) return T2R_ENOMEM;
   p.q = q; p.q_ld = q_ld; p.out = out; p.out_ld = out_ld;
@@ -224,9 +246,8 @@ int t2r_attn_blk_prefill(const void* q, int dtype, int64_t q_ld, const int8_t* k
   BlkAttn p;
   std::memset(&p, 0, sizeof(p));
   if (int rc = cache_args(kc, vc, ks, vs, n_blocks, block, Hk, hd, table, width, &p.c)) return rc;
-  if (!attn_shape_ok(H, Hk) || B <= 0 || rows <= 0 || rows >= kMaxRows || q_ld < (int64_t)H * hd || out_ld < (int64_t)H * hd) return T2R_ESHAPE;
-  const Cut cut = rows_cut(B, rows, H, Hk, hd, block, width);
-  if (cut.nsplit > 65535 || (long long)cut.tiles * Hk > kMaxGroups) return T2R_ESHAPE;
+  Cut cut;
+  if (!rows_sizes(B, rows, H, Hk, hd, block, width, &cut) || q_ld < (int64_t)H * hd || out_ld < (int64_t)H * hd) return T2R_ESHAPE;
   const long long need = rows_ws(cut, Hk, hd);
   if (need > 0 && (!workspace || workspace_bytes < need || misaligned(workspace, 16))) return T2R_ENOMEM;
   p.q = q; p.q_ld = q_ld; p.out = out; p.out_ld = out_ld;
@@ -256,9 +277,8 @@ int t2r_attn_blk_prefill(const void* q, int dtype, int64_t q_ld, const int8_t* k
 }
 
 int64_t t2r_logprobs_workspace_bytes(int rows, int V, int top) {
-  if (rows <= 0 || V <= 0 || top < 0) return -1;
-  const Cut cut = lp_cut(rows, V);
-  return cut.nsplit > 1 ? (long long)rows * cut.nsplit * (16 + 8LL * top) : 0;
+  Cut cut;
+  return top >= 0 && top <= kLpMaxTop && top <= V && lp_sizes(rows, V, &cut) ? lp_ws(cut, rows, top) : -1;
 }
 
 int t2r_logprobs(const void* logits, int dtype, int64_t ld, const int32_t* tokens, int rows, int V, int top,
@@ -268,11 +288,10 @@ int t2r_logprobs(const void* logits, int dtype, int64_t ld, const int32_t* token
   if (misaligned(logits, elem_size(dtype)) || misaligned(tokens, 4) || misaligned(logprob, 4) || misaligned(entropy, 4) ||
       misaligned(top_ids, 4) || misaligned(top_logprob, 4))
     return T2R_EINVAL;
-  if (rows <= 0 || V <= 0 || V > INT32_MAX - 2 * kLpSpan || ld < V) return T2R_ESHAPE;
+  Cut cut;
+  if (!lp_sizes(rows, V, &cut) || ld < V) return T2R_ESHAPE;
   if (top < 0 || top > kLpMaxTop || top > V) return T2R_ERANGE;
-  const Cut cut = lp_cut(rows, V);
-  if ((long long)rows * cut.nsplit > kMaxGroups) return T2R_ESHAPE;
-  const long long need = t2r_logprobs_workspace_bytes(rows, V, top);
+  const long long need = lp_ws(cut, rows, top);
   if (need > 0 && (!workspace || workspace_bytes < need || misaligned(workspace, 16))) return T2R_ENOMEM;
   LpArgs p;
   std::memset(&p, 0, sizeof(p));
