@@ -190,7 +190,9 @@ int t2r_kv_read_blk(const int8_t* kc, const int8_t* vc, const float* ks, const f
 /* Attention over that cache, out = softmax(scale q K^T) V, H / Hk <= 32 query heads a KV head; q [.., H * hd] and out of
  * the same type, q_ld / out_ld elements from row to row (out may be q). scale > 0. A row that sees no position (an idle
  * sequence, or one whose table has no blocks there) gives zeros, one with a NaN in it NaN; what one with an infinity, or
- * with scores past fp32's range, gives is not defined.
+ * with scores past 2 10^6 in size, gives is not defined. As with any softmax in fp32, scores of size A cost a relative error of
+ * some A 2^-22. V scales may lie as far apart as fp32's numbers do: a row's result depends on the blocks that it sees alone, and
+ * is within fp32's range wherever its values' weighted mean is.
  * _decode: row b is sequence b's newest token and sees positions 0 .. lens[b] - 1; B <= 65535, and a table
  * spans less than 2^27 positions.
  * _prefill: ragged rows, each sees the positions up to its own. A row below position 0 (lens[b] less than the sequence's

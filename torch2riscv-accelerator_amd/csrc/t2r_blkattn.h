@@ -8,10 +8,14 @@
 //  - p V's scale, again as two numbers with fp32 rows (the fp32 result then stays within a few 2^-22) and as one with
 //    16-bit ones, whose result keeps 8 or 11 bits.
 // Scores, maxima, sums and outputs are fp32. The scale of a K block multiplies the scores, that of a V block the
-// probabilities: w = p vs / vref with vref the largest vs seen, so that w <= p fits fp16 whatever the scales are.
-// A maximum is raised only where a score passes it by more than a factor 2^kSlack, so that most steps neither rescale nor
-// exchange maxima between lanes. p is kept 2^kLift larger than the maximum says: it reaches 2^(kLift + kSlack), within
-// fp16's range, and fp16's smallest step (2^-25 off) is 2^-36 of a row's largest probability times vref.
+// probabilities, as a power of two in their exponent: with t = log2(e) scale q . k and u = log2 vs a weight is 2^(t + u).
+// The values' sums o run about a base M of the row's own that follows max (t + u), the weights' sum l about another one, m, that
+// follows max t: out = 2^(M - m) o / l. A weight is so held against the largest one that the row itself sees, whatever the scales
+// are, of blocks that it does not see among them; and nothing leaves fp32's range before the division, however large V is.
+// Both bases are whole numbers, so that neither they nor a scale's exponent add a rounding: t is the only large term.
+// M is raised only where a weight passes it by more than a factor 2^kSlack, so that most steps neither rescale nor exchange
+// maxima between lanes. A weight is kept 2^kLift larger than its base says: it reaches 2^(kLift + kSlack), within fp16's range, and
+// fp16's smallest step (2^-25 off) is 2^-36 of the row's largest weight.
 //
 // The MFMA lane layouts meet without any exchange: a lane of S^T holds 4 rows of each 16 (or 4 of each 8 of 32), and
 // which key a row stands for is free. Rows are assigned so that a lane ends up with 16 consecutive keys, which are
@@ -26,7 +30,9 @@ namespace t2r {
 constexpr int kBaThreads = 256, kBaWaves = 4;
 constexpr int kBaSeg = 2048;                 // keys whose table entries and scales lie in LDS at a time
 constexpr float kSlack = 4.0f, kLift = 11.0f;
+constexpr float kFar = 40.0f;                // t above m at which m is raised: l has fp32's range
 constexpr float kNegInf = -__builtin_inff();
+constexpr float kNoBase = -1e30f;            // a base before the first key: any t lies far above it, and differences with it are numbers
 
 T2R_DEV int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
@@ -41,7 +47,7 @@ struct BlkAttn {
   float a;                  // softmax scale times log2(e)
   int order;                // find_piece's, of the tiles
   int chunk, nsplit;        // keys of a workgroup (a multiple of 128 where there are several; the step form: at most kBaSeg)
-  float* ws_o;              // parts of long rows: [row's column, split, hd] sums, and [.., 2] maxima and weights
+  float* ws_o;              // parts of long rows: [row's column, split, hd] sums, and [.., 4] their bases M and m and weights
   float* ws_ml;
 };
 
@@ -82,20 +88,18 @@ T2R_DEV float add_ror8(float x) {
 }
 
 // What a segment's keys need, 16 keys an entry: where their codes begin in kc and in vc (0 where there is no block), how many
-// of them there are, the K scale, and the V scale as a share of vref: its log2, which goes into the probabilities' exponent, and its inverse, which
-// takes it out of their sum again. (A share below 2^-60 counts as that: its values are nothing beside vref's, the
-// probabilities' sum is right all the same.)
+// of them there are, the K scale, and the V scale's u = log2 vs in two: the exponent, a whole number, and the rest in [0, 1).
 struct BaSeg {
   long long k_at[kBaSeg / 16], v_at[kBaSeg / 16];
   int seen[kBaSeg / 16];                      // 16, or fewer at the end, or none
-  float ks[kBaSeg / 16], lw[kBaSeg / 16], iw[kBaSeg / 16];
-  float red[kBaWaves];
+  float ks[kBaSeg / 16], ue[kBaSeg / 16], uf[kBaSeg / 16];
   int holes[kBaWaves];
 };
+constexpr float kNoScale = -512.0f;           // u of a scale of 0: such a block's weights count, its values are nothing
 // The tables of the keys key0 .. key0 + n - 1, in whole steps of `step` keys, for the whole workgroup. In parts, so that what
 // a kernel has to load meanwhile is asked for between them: seg_table asks for this thread's table entry; seg_blocks puts the
-// places into LDS (a barrier: the codes can be asked for then); seg_scales the scales (a second one), and returns the larger
-// of vref and the V scales among them; *holes: some of the n keys have no block.
+// places into LDS (a barrier: the codes can be asked for then); seg_scales the scales (a second one), and returns whether
+// some of the n keys have no block.
 T2R_DEV int seg_table(const BlkCache& c, int b, long long key0, int n) {
   const int tid = threadIdx.x;
   return tid * 16 < n ? c.block(b, (key0 + tid * 16) >> c.lbs) : -1;
@@ -111,7 +115,7 @@ T2R_DEV void seg_blocks(BaSeg& sg, const BlkCache& c, int blk, int head, int n, 
   }
   __syncthreads();
 }
-T2R_DEV float seg_scales(BaSeg& sg, const BlkCache& c, int blk, int head, int n, int step, float vref, bool* holes) {
+T2R_DEV bool seg_scales(BaSeg& sg, const BlkCache& c, int blk, int head, int n, int step) {
   const int tid = threadIdx.x, wave = wave_index(), entries = (n + step - 1) / step * (step >> 4);
   float ks = 0, vs = 0;
   if (blk >= 0) {
@@ -119,30 +123,48 @@ T2R_DEV float seg_scales(BaSeg& sg, const BlkCache& c, int blk, int head, int n,
     ks = c.ks[at];
     vs = c.vs[at];
   }
-  const float wm = wave_max0(fabsf(vs));
   const bool hole = __any(tid * 16 < n && blk < 0);
-  if ((tid & 63) == 0) {
-    sg.red[wave] = wm;
-    sg.holes[wave] = hole;
-  }
-  __syncthreads();
-  float m = vref;
-  int any = 0;
-#pragma unroll
-  for (int w = 0; w < kBaWaves; ++w) {
-    m = fmaxf(m, sg.red[w]);
-    any |= sg.holes[w];
-  }
-  *holes = any != 0;
+  if ((tid & 63) == 0) sg.holes[wave] = hole;
   if (tid < entries) {
     sg.ks[tid] = ks;
-    const float share = m > 0 && blk >= 0 ? fmaxf(vs / m, 0x1p-60f) : 1.0f;
-    sg.lw[tid] = __builtin_amdgcn_logf(share);
-    sg.iw[tid] = 1.0f / share;
+    // (subnormal scales have an exponent, too)
+    sg.ue[tid] = vs > 0 ? (float)(__builtin_amdgcn_frexp_expf(vs) - 1) : kNoScale;
+    sg.uf[tid] = vs > 0 ? __builtin_amdgcn_logf(2.0f * __builtin_amdgcn_frexp_mantf(vs)) : 0.0f;
   }
   __syncthreads();
-  return m;
+  int any = 0;
+#pragma unroll
+  for (int w = 0; w < kBaWaves; ++w) any |= sg.holes[w];
+  return any != 0;
 }
+
+// The bases of a column, the same in each of its lanes.
+struct Bases { float M, m; };
+// A lane's 16 keys of one block, their largest t in tm (-inf: none is seen): raises the bases where needed, and o and l with
+// them. `cols`: f(x) = the largest x of the column's lanes.
+template <int DT, class V, class F> T2R_DEV void raise_bases(float tm, float u, Bases& b, float& l, V* o, F cols) {
+  const float wm = tm + u;
+  if (!__any(wm > b.M + (kLift + kSlack) || tm > b.m + kFar)) return;
+  const float t = cols(tm), w = cols(wm);
+  const float M = w > b.M + (kLift + kSlack) ? floorf(w) - kLift : b.M, m = t > b.m ? floorf(t) : b.m;
+  l *= m == b.m ? 1.0f : __builtin_amdgcn_exp2f(b.m - m);
+  const float f = M == b.M ? 1.0f : __builtin_amdgcn_exp2f(b.M - M);
+#pragma unroll
+  for (int i = 0; i < DT; ++i) o[i] *= f;
+  b = Bases{M, m};
+}
+// What is added to those keys' t: u - M, but at least so much that their largest weight is 2^-60: below that the values add
+// nothing to o (fp16 gives 0 either way), while the weights, with u taken out again, may be all there is to l. At most -kNoBase,
+// where no key is seen.
+T2R_DEV float weight_exponent(float tm, float ue, float uf, const Bases& b) {
+  return __builtin_amdgcn_fmed3f(-60.0f - tm, ue - b.M, -kNoBase) + uf;
+}
+// l and those keys' weights, whose sum is ws: that exponent is taken out again, and m put in
+T2R_DEV float add_weights(float l, float ws, float add, const Bases& b) {
+  return __builtin_fmaf(ws, __builtin_amdgcn_exp2f(-add - b.m), l);
+}
+// 2^(M - m), as ldexp takes it
+T2R_DEV int base_shift(const Bases& b) { return (int)(b.M - b.m); }
 
 // ---------------------------------------------------------------- one row a sequence
 // A workgroup takes `chunk` keys of one (sequence, KV head) and up to HW of its query heads, its four waves every fourth
@@ -159,7 +181,8 @@ template <class E, int HD>
 __global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_step(BlkAttn p) {
   constexpr int NP = Pieces<E>::kN, HW = Pieces<E>::kHeads, KU = HD / 64, DT = HD / 16;
   __shared__ BaSeg sg;
-  __shared__ float s_m[kBaWaves][16], s_l[kBaWaves][16];
+  __shared__ Bases s_b[kBaWaves][16];
+  __shared__ float s_l[kBaWaves][16];
   __shared__ float s_o[kBaWaves][16][HD + 4];
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_index(), col = lane & 15, c4 = lane >> 4;
   const int sets = (p.G + HW - 1) / HW;
@@ -211,8 +234,7 @@ __global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_step(BlkAt
     load_k(st);
     load_v(st);
   }
-  bool holes;
-  const float vref = seg_scales(sg, p.c, mine, kvh, n, 64, 0.0f, &holes);
+  const bool holes = seg_scales(sg, p.c, mine, kvh, n, 64);
   // q's pieces in the layout of K's rows, after the row's largest magnitude
   v8h_t qf[KU][2];
   float sq;
@@ -238,7 +260,8 @@ __global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_step(BlkAt
     }
     sq = p.a * pow2i(e);
   }
-  float m = kNegInf, l = 0;
+  Bases bs{kNoBase, kNoBase};
+  float l = 0;
   v4f_t o[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i) o[i] = v4f_t{0, 0, 0, 0};
@@ -258,7 +281,7 @@ __global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_step(BlkAt
     if (more) load_k(st + kBaWaves);
     // this lane's 16 keys: 16 c4 + 4 t + r of the 64
     const int ch = st * 4 + c4;
-    const float sk = score_scale(sq, sg.ks[ch]), lw = sg.lw[ch], iw = sg.iw[ch];
+    const float sk = score_scale(sq, sg.ks[ch]), ue = sg.ue[ch], uf = sg.uf[ch];
     if (NP == 2) {
 #pragma unroll
       for (int t = 0; t < 4; ++t)
@@ -276,18 +299,11 @@ __global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_step(BlkAt
 #pragma unroll
     for (int t = 1; t < 4; ++t) mx = fmaxf(mx, fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])));
     mx *= sk;
-    if (__any(mx > m + kSlack)) {
-      mx = fmaxf(mx, __shfl_xor(mx, 16));
-      mx = fmaxf(mx, __shfl_xor(mx, 32));
-      if (mx > m + kSlack) {
-        const float al = __builtin_amdgcn_exp2f(m - mx);
-        m = mx;
-        l *= al;
-#pragma unroll
-        for (int i = 0; i < DT; ++i) o[i] *= al;
-      }
-    }
-    const float add = lw + kLift - (m == kNegInf ? 0.0f : m);
+    raise_bases<DT>(mx, ue + uf, bs, l, o, [](float x) {
+      x = fmaxf(x, __shfl_xor(x, 16));
+      return fmaxf(x, __shfl_xor(x, 32));
+    });
+    const float add = weight_exponent(mx, ue, uf, bs);
     v8h_t pf[2];
     float ls[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -303,7 +319,7 @@ __global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_step(BlkAt
         }
         pf[t >> 1][(t & 1) * 4 + r] = h;
       }
-    l = __builtin_fmaf((ls[0] + ls[1]) + (ls[2] + ls[3]), iw, l);
+    l = add_weights(l, (ls[0] + ls[1]) + (ls[2] + ls[3]), add, bs);
 #pragma unroll
     for (int i = 0; i < DT; ++i) {
       o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_h(vr[i][0], vr[i][1]), pf[0], o[i], 0, 0, 0);
@@ -325,63 +341,64 @@ __global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_step(BlkAt
       s_o[wave][col][i * 16 + c4 * 4 + r] = x;
     }
   if (c4 == 0) {
-    s_m[wave][col] = m;
+    s_b[wave][col] = bs;
     s_l[wave][col] = l;
   }
   __syncthreads();
   const bool whole = k0 == 0 && n == len;                 // the only part: the result itself
   for (int i = tid; i < nh * hd; i += kBaThreads) {
     const int h = i / hd, d = i - h * hd;
-    float mm = kNegInf;
+    Bases top{kNoBase, kNoBase};
 #pragma unroll
-    for (int w = 0; w < kBaWaves; ++w) mm = fmaxf(mm, s_m[w][h]);
-    const float mu = mm == kNegInf ? 0.0f : mm;
+    for (int w = 0; w < kBaWaves; ++w) top = Bases{fmaxf(top.M, s_b[w][h].M), fmaxf(top.m, s_b[w][h].m)};
     float x = 0, ls = 0;
 #pragma unroll
     for (int w = 0; w < kBaWaves; ++w) {
-      const float f = __builtin_amdgcn_exp2f(s_m[w][h] - mu);
-      x += f * s_o[w][h][d];
-      ls += f * s_l[w][h];
+      x += __builtin_amdgcn_exp2f(s_b[w][h].M - top.M) * s_o[w][h][d];
+      ls += __builtin_amdgcn_exp2f(s_b[w][h].m - top.m) * s_l[w][h];
     }
-    x *= vref;
     if (whole) {
-      out[i] = narrow<E>(ls == 0 ? 0.0f : x / ls);
+      out[i] = narrow<E>(ls == 0 ? 0.0f : __builtin_amdgcn_ldexpf(x / ls, base_shift(top)));
     } else {
       const long long at = ((long long)b * p.H + kvh * p.G + h0 + h) * p.nsplit + split;
       p.ws_o[at * hd + d] = x;
-      if (d == 0) {
-        p.ws_ml[2 * at] = mm;
-        p.ws_ml[2 * at + 1] = ls;
-      }
+      if (d == 0) *(v4f_t*)(p.ws_ml + 4 * at) = v4f_t{top.M, top.m, ls, 0};
     }
   }
 }
 
-// Joins the parts of a row: their sums, moved to the largest of their maxima. NWV waves of the workgroup take every NWV-th part
-// each, a lane two channels; what the row's first wave has in *x is the row (and the weights' sum, the same in every wave, comes
-// back). The parts' maxima are read 64 at a time, a lane each; the sums' loads wait for nothing. A wave has eight parts' sums
+// Joins the parts of a row: their sums, moved to the largest of their bases. NWV waves of the workgroup take every NWV-th part
+// each, a lane two channels; what the row's first wave has in *x is the row (and the weights' sum and the bases, the same in every
+// wave, come back). The parts' bases are read 64 at a time, a lane each; the sums' loads wait for nothing. A wave has eight parts' sums
 // in flight, and eight more cost a memory's latency: from kJoinWide parts on a row is worth four waves (32 columns of 32
 // heads in 13 / 32 parts: 6.5 / 9.4 us with a wave each).
 constexpr int kJoinWide = 9;
 template <int NWV>
-T2R_DEV float join_parts(const BlkAttn& p, long long at, int parts, float (*x)[2]) {
+T2R_DEV float join_parts(const BlkAttn& p, long long at, int parts, float (*x)[2], Bases* top) {
   __shared__ float s_x[NWV > 1 ? kBaWaves : 1][64][2];
   const int lane = threadIdx.x & 63, hd = p.c.hd, d = min(2 * lane, hd - 2), wave = NWV > 1 ? wave_index() : 0;
   typedef float v2f_t __attribute__((ext_vector_type(2)));
-  const v2f_t* ml = (const v2f_t*)p.ws_ml + at;
-  float mm = kNegInf;
-  for (int s = lane; s < parts; s += 64) mm = fmaxf(mm, ml[s][0]);
+  const v4f_t* ml = (const v4f_t*)p.ws_ml + at;
+  float M = kNoBase, m = kNoBase;
+  for (int s = lane; s < parts; s += 64) {
+    const v4f_t v = ml[s];
+    M = fmaxf(M, v[0]);
+    m = fmaxf(m, v[1]);
+  }
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o));
-  const float mu = mm == kNegInf ? 0.0f : mm;
+  for (int o = 32; o > 0; o >>= 1) {
+    M = fmaxf(M, __shfl_xor(M, o));
+    m = fmaxf(m, __shfl_xor(m, o));
+  }
+  *top = Bases{M, m};
   float l = 0;
   v2f_t y = {0, 0};
   for (int b = 0; b < parts; b += 64) {
     const int n = min(parts - b, 64);
-    v2f_t v = {kNegInf, 0};
+    v4f_t v = {kNoBase, kNoBase, 0, 0};
     if (lane < n) v = ml[b + lane];
-    const float f = __builtin_amdgcn_exp2f(v[0] - mu);
-    l += f * v[1];
+    const float f = __builtin_amdgcn_exp2f(v[0] - M);
+    l += __builtin_amdgcn_exp2f(v[1] - m) * v[2];
     const float* o = p.ws_o + (at + b) * hd + d;
 #pragma unroll 8
     for (int s = wave; s < n; s += NWV) y += fv((uint32_t)__builtin_amdgcn_readlane((int)fb(f), s)) * *(const v2f_t*)(o + s * hd);
@@ -404,12 +421,13 @@ T2R_DEV float join_parts(const BlkAttn& p, long long at, int parts, float (*x)[2
 }
 // two channels of a joined row; place: it stands in its sequence
 template <class E>
-T2R_DEV void join_store(const BlkAttn& p, E* out, const float* x, float l, bool place) {
+T2R_DEV void join_store(const BlkAttn& p, E* out, const float* x, float l, const Bases& top, bool place) {
   const int d = 2 * (threadIdx.x & 63);
   if (d >= p.c.hd) return;
   const float inv = !place ? fv(kQNaN) : l == 0 ? 0.0f : 1.0f / l;
-  out[d] = narrow<E>(x[0] * inv);
-  out[d + 1] = narrow<E>(x[1] * inv);
+  const int e = base_shift(top);
+  out[d] = narrow<E>(__builtin_amdgcn_ldexpf(x[0] * inv, e));
+  out[d + 1] = narrow<E>(__builtin_amdgcn_ldexpf(x[1] * inv, e));
 }
 
 // a workgroup per (head, sequence); 4.3 us, 3.3 of them an empty kernel's
@@ -420,8 +438,9 @@ __global__ __launch_bounds__(kBaThreads) void k_blk_step_join(BlkAttn p) {
   if (len <= p.chunk) return;                             // one part (or none): written already
   const int parts = (int)((len + p.chunk - 1) / p.chunk);
   float x[2];
-  const float l = join_parts<kBaWaves>(p, ((long long)b * p.H + h) * p.nsplit, parts, &x);
-  if (wave_index() == 0) join_store<E>(p, (E*)p.out + (long long)b * p.out_ld + (long long)h * p.c.hd, x, l, true);
+  Bases top;
+  const float l = join_parts<kBaWaves>(p, ((long long)b * p.H + h) * p.nsplit, parts, &x, &top);
+  if (wave_index() == 0) join_store<E>(p, (E*)p.out + (long long)b * p.out_ld + (long long)h * p.c.hd, x, l, top, true);
 }
 
 // ---------------------------------------------------------------- several rows a sequence
@@ -499,9 +518,9 @@ T2R_DEV float q_pieces(int hd, const float (*x)[16], v8h_t (*qf)[Pieces<E>::kN][
 }
 
 // The softmax of 32 keys' scores s for a lane's column: this lane's 16 keys are 16 (lane / 32) + r, `left` of them (below 16
-// only if EDGE) are seen. First the maximum, raised where needed (o and l with it) ...
+// only if EDGE) are seen. First the bases, raised where needed (o and l with them); returns the weights' exponent ...
 template <int DT, bool EDGE>
-T2R_DEV void soft_max(v16f_t& s, float sk, int left, float& m, float& l, v16f_t* o) {
+T2R_DEV float soft_max(v16f_t& s, float sk, int left, float ue, float uf, Bases& b, float& l, v16f_t* o) {
   if constexpr (EDGE) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = r < left ? s[r] : kNegInf;
@@ -510,17 +529,10 @@ T2R_DEV void soft_max(v16f_t& s, float sk, int left, float& m, float& l, v16f_t*
 #pragma unroll
   for (int r = 2; r < 16; r += 2) mx = fmaxf(fmaxf(mx, s[r]), s[r + 1]);
   mx *= sk;
-  if (__any(mx > m + kSlack)) {
-    mx = fmaxf(mx, __shfl_xor(mx, 32));
-    const float n = mx > m + kSlack ? mx : m;
-    const float al = n == m ? 1.0f : __builtin_amdgcn_exp2f(m - n);
-    m = n;
-    l *= al;
-#pragma unroll
-    for (int i = 0; i < DT; ++i) o[i] *= al;
-  }
+  raise_bases<DT>(mx, ue + uf, b, l, o, [](float x) { return fmaxf(x, __shfl_xor(x, 32)); });
+  return weight_exponent(mx, ue, uf, b);
 }
-// ... then the probabilities: those of keys r .. r + 3, times their V block's share, as fp16 pieces, and their sum; ...
+// ... then the weights of keys r .. r + 3 as fp16 pieces, and their sum; ...
 template <int NP>
 T2R_DEV float soft_weights(const v16f_t& s, float sk, float add, v8h_t (*pf)[2], int r) {
   typedef float v2f_t __attribute__((ext_vector_type(2)));
@@ -546,12 +558,11 @@ T2R_DEV float soft_weights(const v16f_t& s, float sk, float add, v8h_t (*pf)[2],
 }
 // ... of all 16, and their sum into l.
 template <int NP>
-T2R_DEV void soft_exp(const v16f_t& s, float sk, float lw, float iw, float m, float& l, v8h_t (*pf)[2]) {
-  const float add = lw + kLift - (m == kNegInf ? 0.0f : m);
+T2R_DEV void soft_exp(const v16f_t& s, float sk, float add, const Bases& b, float& l, v8h_t (*pf)[2]) {
   float ls = 0;
 #pragma unroll
   for (int r = 0; r < 16; r += 4) ls += soft_weights<NP>(s, sk, add, pf, r);
-  l = __builtin_fmaf(ls, iw, l);
+  l = add_weights(l, ls, add, b);
 }
 
 // The end of a tile: its waves' sums (wave's column group cg of 32 CT, key group kg of KG) are joined through LDS (so: KG x COLS
@@ -559,7 +570,7 @@ T2R_DEV void soft_exp(const v16f_t& s, float sk, float lw, float iw, float m, fl
 // keys, into the workspace.
 template <int HD, int CT, int CG> struct TileEnd {
   static constexpr int KG = kBaWaves / CG, COLS = 32 * CT * CG, LD = HD + 4, kBytes = KG * COLS * LD * 4;
-  struct Ml { float m[KG][COLS], l[KG][COLS], top[COLS], sum[COLS], inv[COLS]; };
+  struct Ml { Bases b[KG][COLS], top[COLS]; float l[KG][COLS], sum[COLS], inv[COLS]; };
 };
 // four values side by side, at any element's alignment
 template <class E> T2R_DEV void store4(E* p, v4f_t x) {
@@ -567,7 +578,7 @@ template <class E> T2R_DEV void store4(E* p, v4f_t x) {
   *(V*)p = V{{narrow<E>(x[0]), narrow<E>(x[1]), narrow<E>(x[2]), narrow<E>(x[3])}};
 }
 template <class E, int HD, int CT, int CG>
-T2R_DEV void tile_end(const BlkAttn& p, const Tile& t, int kvh, int split, bool whole, float vref, float* m, float* l,
+T2R_DEV void tile_end(const BlkAttn& p, const Tile& t, int kvh, int split, bool whole, const Bases* b, float* l,
                       v16f_t (*o)[HD / 32], typename TileEnd<HD, CT, CG>::Ml& ml, float* so) {
   using T = TileEnd<HD, CT, CG>;
   constexpr int KG = T::KG, COLS = T::COLS, LD = T::LD, DT = HD / 32;
@@ -577,30 +588,30 @@ T2R_DEV void tile_end(const BlkAttn& p, const Tile& t, int kvh, int split, bool 
   for (int ct = 0; ct < CT; ++ct) {
     l[ct] += __shfl_xor(l[ct], 32);
     if (c2 == 0) {
-      ml.m[kg][(cg * CT + ct) * 32 + col] = m[ct];
+      ml.b[kg][(cg * CT + ct) * 32 + col] = b[ct];
       ml.l[kg][(cg * CT + ct) * 32 + col] = l[ct];
     }
   }
   __syncthreads();
-  // a column's largest maximum over its key groups, and the sum about it
+  // a column's largest bases over its key groups, and the weights' sum about them
   if (tid < COLS) {
-    float mm = ml.m[0][tid], ls = 0;
+    Bases top = ml.b[0][tid];
 #pragma unroll
-    for (int w = 1; w < KG; ++w) mm = fmaxf(mm, ml.m[w][tid]);
-    const float mu = mm == kNegInf ? 0.0f : mm;
+    for (int w = 1; w < KG; ++w) top = Bases{fmaxf(top.M, ml.b[w][tid].M), fmaxf(top.m, ml.b[w][tid].m)};
+    float ls = 0;
 #pragma unroll
-    for (int w = 0; w < KG; ++w) ls += __builtin_amdgcn_exp2f(ml.m[w][tid] - mu) * ml.l[w][tid];
-    ml.top[tid] = mm;
+    for (int w = 0; w < KG; ++w) ls += __builtin_amdgcn_exp2f(ml.b[w][tid].m - top.m) * ml.l[w][tid];
+    ml.top[tid] = top;
     ml.sum[tid] = ls;
     ml.inv[tid] = t.s.p0 + t.i0 + min(tid, ncol - 1) / G < 0 ? fv(kQNaN) : ls == 0 ? 0.0f : 1.0f / ls;
   }
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     const int cc = (cg * CT + ct) * 32 + col;
-    float mm = ml.m[0][cc];
+    float M = ml.b[0][cc].M;
 #pragma unroll
-    for (int w = 1; w < KG; ++w) mm = fmaxf(mm, ml.m[w][cc]);
-    const float f = __builtin_amdgcn_exp2f(m[ct] - (mm == kNegInf ? 0.0f : mm)) * vref;
+    for (int w = 1; w < KG; ++w) M = fmaxf(M, ml.b[w][cc].M);
+    const float f = __builtin_amdgcn_exp2f(b[ct].M - M);
 #pragma unroll
     for (int i = 0; i < DT; ++i)
 #pragma unroll
@@ -619,14 +630,15 @@ T2R_DEV void tile_end(const BlkAttn& p, const Tile& t, int kvh, int split, bool 
 #pragma unroll
     for (int w = 1; w < KG; ++w) x += *(const v4f_t*)(so + (w * COLS + cc) * LD + d);
     if (whole) {
-      store4((E*)p.out + col_at(t, G, hd, kvh, cc, p.out_ld) + d, x * ml.inv[cc]);
+      const int e = base_shift(ml.top[cc]);
+      x *= ml.inv[cc];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = __builtin_amdgcn_ldexpf(x[i], e);
+      store4((E*)p.out + col_at(t, G, hd, kvh, cc, p.out_ld) + d, x);
     } else {
       const long long at = ((long long)blockIdx.x * COLS + cc) * p.nsplit + split;
       *(v4f_t*)(p.ws_o + at * hd + d) = x;
-      if (d == 0) {
-        p.ws_ml[2 * at] = ml.top[cc];
-        p.ws_ml[2 * at + 1] = ml.sum[cc];
-      }
+      if (d == 0) *(v4f_t*)(p.ws_ml + 4 * at) = v4f_t{ml.top[cc].M, ml.top[cc].m, ml.sum[cc], 0};
     }
   }
 }
@@ -680,7 +692,8 @@ __global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_few(BlkAtt
   const long long at = t.s.p0 + t.i0 + cc / G, all_see = t.s.p0 + t.i0 + 1;   // (keys below all_see are seen by every row)
   // row 8 i + 4 c' + r of the 32 stands for key 16 c' + 4 i + r
   const int kc = (col >> 2) & 1, krow = 4 * (col >> 3) + (col & 3);
-  float m = kNegInf, l = 0, vref = 0;
+  Bases bs{kNoBase, kNoBase};
+  float l = 0;
   v16f_t o[1][DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i) o[0][i] = v16f_t{};
@@ -710,13 +723,7 @@ __global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_few(BlkAtt
   const float sq = p.a * q_pieces<E, KU>(hd, x, qf);
   for (long long seg = k0; seg < kend; seg += kBaSeg) {
     const int n = (int)min((long long)kBaSeg, kend - seg), steps = (n + 31) >> 5;
-    bool holes;
-    const float vmax = seg_scales(sg, p.c, blk, kvh, n, 32, vref, &holes);
-    if (vmax > vref) {
-#pragma unroll
-      for (int i = 0; i < DT; ++i) o[0][i] *= vref / vmax;
-    }
-    vref = vmax;
+    const bool holes = seg_scales(sg, p.c, blk, kvh, n, 32);
     int st = wave;
     auto step = [&](auto edge) {
       v16f_t s = {};
@@ -733,8 +740,9 @@ __global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_few(BlkAtt
       const int ch = st * 2 + c2;
       v8h_t pf[NP][2];
       const float sk = score_scale(sq, sg.ks[ch]);
-      soft_max<DT, edge.value>(s, sk, edge.value ? keys_left(at, seg + ch * 16, sg.seen[ch]) : 16, m, l, o[0]);
-      soft_exp<NP>(s, sk, sg.lw[ch], sg.iw[ch], m, l, pf);
+      const float add = soft_max<DT, edge.value>(s, sk, edge.value ? keys_left(at, seg + ch * 16, sg.seen[ch]) : 16, sg.ue[ch],
+                                                 sg.uf[ch], bs, l, o[0]);
+      soft_exp<NP>(s, sk, add, bs, l, pf);
 #pragma unroll
       for (int i = 0; i < DT; ++i)
 #pragma unroll
@@ -755,7 +763,7 @@ __global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_few(BlkAtt
       begin(m);
     }
   }
-  tile_end<E, HD, 1, 1>(p, t, kvh, blockIdx.y, k0 == 0 && kend == t.end, vref, &m, &l, o, ml, (float*)s_o);
+  tile_end<E, HD, 1, 1>(p, t, kvh, blockIdx.y, k0 == 0 && kend == t.end, &bs, &l, o, ml, (float*)s_o);
 }
 
 // LDS of k_blk_tile, in 16-byte slots: a fragment (64 lanes' operand of one MFMA) is 64 slots. K's fragments of a stage are
@@ -784,7 +792,8 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
   const int ncol = t.rows * G;
   int blk = seg_table(p.c, t.s.b, k0, (int)min((long long)kBaSeg, kend - k0));
   v8h_t qf[CT][KU][NP][2];
-  float x[CT][KU][16], sq[CT], m[CT], l[CT], vref = 0;
+  float x[CT][KU][16], sq[CT], l[CT];
+  Bases bs[CT];
   long long at[CT];
   v16f_t o[CT][DT];
 #pragma unroll
@@ -792,7 +801,7 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
     const int cc = min((cg * CT + ct) * 32 + col, ncol - 1);
     q_load<E, KU>((const E*)p.q + col_at(t, G, hd, kvh, cc, p.q_ld), hd, x[ct]);
     at[ct] = t.s.p0 + t.i0 + cc / G;
-    m[ct] = kNegInf;
+    bs[ct] = Bases{kNoBase, kNoBase};
     l[ct] = 0;
 #pragma unroll
     for (int i = 0; i < DT; ++i) o[ct][i] = v16f_t{};
@@ -843,15 +852,7 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
   for (int ct = 0; ct < CT; ++ct) sq[ct] = p.a * q_pieces<E, KU>(hd, x[ct], qf[ct]);
   for (long long seg = k0; seg < kend; seg += kBaSeg) {
     const int n = (int)min((long long)kBaSeg, kend - seg), stages = (n + STAGE - 1) / STAGE, last = stages - 1;
-    bool holes;
-    const float vmax = seg_scales(sg, p.c, blk, kvh, n, STAGE, vref, &holes);
-    if (vmax > vref) {
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-        for (int i = 0; i < DT; ++i) o[ct][i] *= vref / vmax;
-    }
-    vref = vmax;
+    const bool holes = seg_scales(sg, p.c, blk, kvh, n, STAGE);
     // (past the last stage loads repeat it, and nobody reads what is put of them)
 #pragma unroll
     for (int h = 0; h < 4 * PER; ++h) put_half(0, h);
@@ -869,7 +870,7 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
           for (int half = 0; half < 2; ++half) kf[u][half] = buf[((kg * KU + u) * 2 + half) * 64 + (lane ^ ((2 * u + c2) & 7))];
       };
       read_k(0, KU / 2);                                      // (the others follow while these are used)
-      const float ks = sg.ks[ch], lw = sg.lw[ch], iw = sg.iw[ch];
+      const float ks = sg.ks[ch], ue = sg.ue[ch], uf = sg.uf[ch];
       const int seen = edge.value ? sg.seen[ch] : 16;
       __builtin_amdgcn_sched_barrier(0);
       // The scores; between their products the next stage's codes are converted. (The order is pinned: left to itself the
@@ -901,8 +902,8 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
         sk[ct] = score_scale(sq[ct], ks);
-        soft_max<DT, edge.value>(s[ct], sk[ct], edge.value ? keys_left(at[ct], seg + ch * 16, seen) : 16, m[ct], l[ct], o[ct]);
-        add[ct] = lw + kLift - (m[ct] == kNegInf ? 0.0f : m[ct]);
+        add[ct] = soft_max<DT, edge.value>(s[ct], sk[ct], edge.value ? keys_left(at[ct], seg + ch * 16, seen) : 16, ue, uf, bs[ct],
+                                           l[ct], o[ct]);
         ls[ct] = 0;
       }
       // The probabilities of 8 keys, then their products; the other 8 keys' between those, the next loads between the last.
@@ -932,7 +933,7 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
           __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) l[ct] = __builtin_fmaf(ls[ct], iw, l[ct]);
+      for (int ct = 0; ct < CT; ++ct) l[ct] = add_weights(l[ct], ls[ct], add[ct], bs[ct]);
       __syncthreads();                                        // this buffer is read, the other one whole
     };
     const int plain = plain_steps(all_see, seg, n, STAGE, holes);
@@ -946,7 +947,7 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
       begin(m2);
     }
   }
-  tile_end<E, HD, CT, CG>(p, t, kvh, blockIdx.y, k0 == 0 && kend == t.end, vref, m, l, o, ml, (float*)s_big);
+  tile_end<E, HD, CT, CG>(p, t, kvh, blockIdx.y, k0 == 0 && kend == t.end, bs, l, o, ml, (float*)s_big);
 }
 
 // Joins the parts of a tile's columns, NWV waves a column
@@ -959,9 +960,10 @@ __global__ __launch_bounds__(kBaThreads) void k_blk_rows_join(BlkAttn p, int col
   if (cc >= t.rows * p.G) return;
   const int parts = (int)((t.end + p.chunk - 1) / p.chunk);
   float x[2];
-  const float l = join_parts<NWV>(p, ((long long)blockIdx.x * cols + cc) * p.nsplit, parts, &x);
+  Bases top;
+  const float l = join_parts<NWV>(p, ((long long)blockIdx.x * cols + cc) * p.nsplit, parts, &x, &top);
   if (NWV == 1 || wave_index() == 0)
-    join_store<E>(p, (E*)p.out + col_at(t, p.G, p.c.hd, kvh, cc, p.out_ld), x, l, t.s.p0 + t.i0 + cc / p.G >= 0);
+    join_store<E>(p, (E*)p.out + col_at(t, p.G, p.c.hd, kvh, cc, p.out_ld), x, l, top, t.s.p0 + t.i0 + cc / p.G >= 0);
 }
 
 }  // namespace t2r

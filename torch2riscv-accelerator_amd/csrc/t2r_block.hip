@@ -131,7 +131,7 @@ bool rows_sizes(int B, int rows, int H, int Hk, int hd, int block, int width, Cu
   *c = rows_cut(B, rows, H, Hk, hd, block, width);
   return c->nsplit <= 65535 && (long long)c->tiles * Hk <= kMaxGroups;
 }
-long long part_bytes(long long parts, int hd) { return parts * 4 * (hd + 2); }
+long long part_bytes(long long parts, int hd) { return parts * 4 * (hd + 4); }
 long long step_ws(const Cut& c, int B, int H, int hd) { return c.nsplit > 1 ? part_bytes((long long)B * H * c.nsplit, hd) : 0; }
 long long rows_ws(const Cut& c, int Hk, int hd) {
   return c.nsplit > 1 ? part_bytes((long long)c.tiles * Hk * c.cols * c.nsplit, hd) : 0;
