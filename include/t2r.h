@@ -162,7 +162,8 @@ int t2r_argmax(const float* x, int rows, int n, int32_t* idx, void* stream);
 
 /* ------------------------------------------- the block-scaled KV cache and what a caller asks of logits
  * No counterpart in the reference, whose cache has one calibrated scale a layer (or channel). Values are fp32, bf16 or
- * fp16 (dtype below); sums, softmax statistics and scales are fp32. */
+ * fp16 (dtype below); sums, softmax statistics and scales are fp32. The attention's products take q and the softmax's weights as
+ * fp16 numbers, two of them (22 bits) each; one for q of 16 bits, and for the weights of _prefill's bf16 rows (11 bits). */
 enum { T2R_F32 = 0, T2R_BF16 = 1, T2R_F16 = 2 };
 /* The cache: int8 codes in a pool of n_blocks blocks of `block` tokens (16, 32, 64 or 128) with one fp32 scale for each
  * block and KV head, and a table of which block holds which tokens of a sequence:

@@ -188,3 +188,30 @@ def test_scores_up_to_millions(env, form, dtype):
     # to that once, in o and not in l: up to 2^(2^-3) - 1 = 0.0906 of the result (the term A 2^-22 of rows_of at this A is 0.45).
     tol = np.abs(y) * (0.0906 + 2.0 ** -10)
     compare(got, {r: (y, tol) for r in (0, rows - 1)}, dtype)
+
+
+@pytest.mark.parametrize("form,dtype", [("step", "f16"), ("step", "bf16"), ("step of wide groups", "f16"), ("step of wide groups", "bf16"),
+                                        ("few", "f16"), ("few, hd 128", "f16"), ("tile", "f16"), ("tile, hd 128", "f16"),
+                                        ("wide tile", "f16")])
+def test_weights_keep_their_bits_in_16_bit_rows(env, form, dtype):
+    """Rows of 16 bits whose weights are held in two fp16 pieces, as fp32 rows' are: the result is the exact one rounded once, up
+    to fp32's own errors. (q in one piece loses 2^-25 of a row's largest value where a value is small: below A 2^-22 in a score.)"""
+    torch, ops = env
+    H, Hk, hd, n, rows = {"step": (32, 8, 64, 400, 1), "step of wide groups": (32, 2, 128, 300, 1), "few": (8, 2, 64, 300, 8),
+                          "few, hd 128": (8, 2, 128, 300, 8), "tile": (8, 2, 64, 200, 150), "tile, hd 128": (8, 4, 128, 200, 150),
+                          "wide tile": (32, 8, 64, 2200, 2100)}[form]
+    rng = np.random.default_rng(61)
+    c = Both(torch, ops, rng, [n], Hk, hd, 64).fill(rng).send()
+    x, t = rounded(torch, rng.standard_normal((rows, H * hd)), dtype)
+    if form.startswith("step"):
+        got = ops.attention_block(t, *c.dev, c.lens_d, H)
+    else:
+        got = ops.attention_block_prefill(t, *c.dev, i32(torch, [0, rows]), c.lens_d, H)
+    only = range(rows) if rows <= 8 else (0, 1, 33, rows // 2, rows - 2, rows - 1)
+    for r, (y, tol) in rows_of(c, x, 0, rows, H, 1 / math.sqrt(hd), only, 0).items():
+        # (between the roundings of the exact value less and more what fp32 is off; 2^-24 of it: the result's own rounding to fp32)
+        tol = tol + np.abs(y) * 2.0 ** -24
+        lo, hi = (rounded(torch, v, dtype)[0] for v in (y - tol, y + tol))
+        g = got[r].double().cpu().numpy()
+        bad = (g < lo) | (g > hi)
+        assert not bad.any(), (r, int(bad.sum()), g[bad][:3], y[bad][:3], tol[bad][:3])

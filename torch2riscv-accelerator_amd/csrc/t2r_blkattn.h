@@ -3,10 +3,11 @@
 //
 // Both products run on fp16 MFMA with the key axis as the rows: S^T = K Q^T and O^T = V^T P^T. The codes are exact in
 // fp16, and so nothing of the cache is rounded. What is rounded to fp16:
-//  - q, scaled by a power of two to [1, 2) per row: fp32 rows as the sum of two fp16 numbers (22 bits, 2^-25 of the
-//    row's largest value), 16-bit rows as one (exact but for values below 2^-24 of it);
-//  - p V's scale, again as two numbers with fp32 rows (the fp32 result then stays within a few 2^-22) and as one with
-//    16-bit ones, whose result keeps 8 or 11 bits.
+//  - q, scaled by a power of two to [1, 2) per row: fp32 rows as the sum of two fp16 numbers (22 bits), 16-bit rows as one;
+//    either way 2^-25 of the row's largest value is lost at most (nothing of fp16 values down to 2^-14 of it, of bf16 ones down
+//    to 2^-17);
+//  - the weights, p times V's scale, again as two numbers (the fp32 result then stays within a few 2^-22), but as one in the ragged
+//    form's bf16 rows (Pieces).
 // Scores, maxima, sums and outputs are fp32. The scale of a K block multiplies the scores, that of a V block the
 // probabilities, as a power of two in their exponent: with t = log2(e) scale q . k and u = log2 vs a weight is 2^(t + u).
 // The values' sums o run about a base M of the row's own that follows max (t + u), the weights' sum l about another one, m, that
@@ -169,17 +170,23 @@ T2R_DEV int base_shift(const Bases& b) { return (int)(b.M - b.m); }
 // ---------------------------------------------------------------- one row a sequence
 // A workgroup takes `chunk` keys of one (sequence, KV head) and up to HW of its query heads, its four waves every fourth
 // 64 of them. 16 x 16 x 32 MFMA: columns 0 .. HW - 1 are the heads; with fp32 rows columns 8 .. 15 hold their low
-// pieces, so that one product serves both and the columns are added afterwards.
+// pieces, so that one product serves both and the columns are added afterwards. 16-bit rows have 16 heads and a second product of
+// the weights' low pieces.
 //
 // Every code is needed once, so the codes go from memory into the waves' registers, a step ahead, and never through LDS; the
 // loads of a step are 64 tokens' whole rows. Long caches are bound by memory: 32 sequences of 8192 tokens, 8 KV heads of 128,
 // 5.4 TB/s; of 1021 .. 8192 tokens 63 us (4.8 TB/s: the longest sequences end alone) and 4.3 for the join. Short ones are a
 // chain of length, table, scales, codes and products: one sequence of 96 tokens 4.5 us, of 8101 5.9 and 4.4.
-template <class E> struct Pieces { static constexpr int kN = sizeof(E) == 4 ? 2 : 1, kHeads = 16 / kN; };
+//
+// fp16 pieces of an fp32 number: of q, of the weights of the ragged form. One piece of a weight is 2^-12 off, which fp16 results
+// show (2-norm, 2.9e-4 off against 2.06e-4 of the rounded exact ones and of two pieces) and bf16's do not (1.67e-3, 1.65e-3,
+// 1.65e-3). A second one costs the tiles 15 to 19% (2032 rows, 32 heads of 64: 39.7 and 45.9 us; 16 of 128: 40.4 and 46.5), so bf16
+// rows have one there. The step form, bound by memory, always has two: 0 to 4%.
+template <class E> struct Pieces { static constexpr int kQ = sizeof(E) == 4 ? 2 : 1, kW = std::is_same<E, bf16_t>::value ? 1 : 2; };
 
 template <class E, int HD>
 __global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_step(BlkAttn p) {
-  constexpr int NP = Pieces<E>::kN, HW = Pieces<E>::kHeads, KU = HD / 64, DT = HD / 16;
+  constexpr int NQ = Pieces<E>::kQ, NP = 3 - NQ, HW = 16 / NQ, KU = HD / 64, DT = HD / 16;     // NP: operands of weights
   __shared__ BaSeg sg;
   __shared__ Bases s_b[kBaWaves][16];
   __shared__ float s_l[kBaWaves][16];
@@ -254,7 +261,7 @@ __global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_step(BlkAt
       for (int i = 0; i < 16; ++i) {
         const float y = held(x[u][i] * down);
         _Float16 h = (_Float16)y;
-        if (NP == 2 && col >= 8) h = (_Float16)(y - (float)h);
+        if (NQ == 2 && col >= 8) h = (_Float16)(y - (float)h);
         qf[u][i >> 3][i & 7] = h;
       }
     }
@@ -282,7 +289,7 @@ __global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_step(BlkAt
     // this lane's 16 keys: 16 c4 + 4 t + r of the 64
     const int ch = st * 4 + c4;
     const float sk = score_scale(sq, sg.ks[ch]), ue = sg.ue[ch], uf = sg.uf[ch];
-    if (NP == 2) {
+    if (NQ == 2) {
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -304,7 +311,7 @@ __global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_step(BlkAt
       return fmaxf(x, __shfl_xor(x, 32));
     });
     const float add = weight_exponent(mx, ue, uf, bs);
-    v8h_t pf[2];
+    v8h_t pf[NP][2];
     float ls[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int t = 0; t < 4; ++t)
@@ -312,19 +319,19 @@ __global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_step(BlkAt
       for (int r = 0; r < 4; ++r) {
         const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][r], sk, add));
         ls[r] += w;
-        _Float16 h = (_Float16)w;
-        if (NP == 2) {
-          const _Float16 lo = (_Float16)__builtin_fmaf((float)h, -1.0f, w);
-          h = col >= 8 ? lo : h;
-        }
-        pf[t >> 1][(t & 1) * 4 + r] = h;
+        const _Float16 h = (_Float16)w, lo = (_Float16)__builtin_fmaf((float)h, -1.0f, w);
+        pf[0][t >> 1][(t & 1) * 4 + r] = NQ == 2 && col >= 8 ? lo : h;
+        if (NP == 2) pf[NP - 1][t >> 1][(t & 1) * 4 + r] = lo;
       }
     l = add_weights(l, (ls[0] + ls[1]) + (ls[2] + ls[3]), add, bs);
 #pragma unroll
-    for (int i = 0; i < DT; ++i) {
-      o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_h(vr[i][0], vr[i][1]), pf[0], o[i], 0, 0, 0);
-      o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_h(vr[i][2], vr[i][3]), pf[1], o[i], 0, 0, 0);
-    }
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const v8h_t vf = codes_h(vr[i][2 * half], vr[i][2 * half + 1]);
+#pragma unroll
+        for (int q = 0; q < NP; ++q) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[q][half], o[i], 0, 0, 0);
+      }
     if (more) load_v(st + kBaWaves);
   };
   for (const int plain = holes ? 0 : n >> 6; st < plain; st += kBaWaves) step(std::false_type());
@@ -337,7 +344,7 @@ __global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_step(BlkAt
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       float x = o[i][r];
-      if (NP == 2) x = add_ror8(x);
+      if (NQ == 2) x = add_ror8(x);
       s_o[wave][col][i * 16 + c4 * 4 + r] = x;
     }
   if (c4 == 0) {
@@ -493,8 +500,8 @@ T2R_DEV void q_load(const E* q, int hd, float (*x)[16]) {
 }
 // ... and as fp16 pieces (zero past hd), in the order of K's rows; returns 2^e of the power that was taken out
 template <class E, int KU>
-T2R_DEV float q_pieces(int hd, const float (*x)[16], v8h_t (*qf)[Pieces<E>::kN][2]) {
-  constexpr int NP = Pieces<E>::kN;
+T2R_DEV float q_pieces(int hd, const float (*x)[16], v8h_t (*qf)[Pieces<E>::kQ][2]) {
+  constexpr int NQ = Pieces<E>::kQ;
   const int c2 = (threadIdx.x & 63) >> 5;
   float am = 0;
 #pragma unroll
@@ -511,7 +518,7 @@ T2R_DEV float q_pieces(int hd, const float (*x)[16], v8h_t (*qf)[Pieces<E>::kN][
       const float y = held(x[u][i] * down);
       const _Float16 h = (_Float16)y;
       qf[u][0][i >> 3][i & 7] = h;
-      if (NP == 2) qf[u][NP - 1][i >> 3][i & 7] = (_Float16)__builtin_fmaf((float)h, -1.0f, y);
+      if (NQ == 2) qf[u][NQ - 1][i >> 3][i & 7] = (_Float16)__builtin_fmaf((float)h, -1.0f, y);
     }
   }
   return pow2i(e);
@@ -533,7 +540,7 @@ T2R_DEV float soft_max(v16f_t& s, float sk, int left, float ue, float uf, Bases&
   return weight_exponent(mx, ue, uf, b);
 }
 // ... then the weights of keys r .. r + 3 as fp16 pieces, and their sum; ...
-template <int NP>
+template <int NW>
 T2R_DEV float soft_weights(const v16f_t& s, float sk, float add, v8h_t (*pf)[2], int r) {
   typedef float v2f_t __attribute__((ext_vector_type(2)));
   float w[4];
@@ -549,19 +556,19 @@ T2R_DEV float soft_weights(const v16f_t& s, float sk, float add, v8h_t (*pf)[2],
     asm("" : "+s"(minus));
     pf[0][r >> 3][(r & 7) + i] = h[0];
     pf[0][r >> 3][(r & 7) + i + 1] = h[1];
-    if (NP == 2) {
-      pf[NP - 1][r >> 3][(r & 7) + i] = (_Float16)__builtin_fmaf((float)h[0], minus, w[i]);
-      pf[NP - 1][r >> 3][(r & 7) + i + 1] = (_Float16)__builtin_fmaf((float)h[1], minus, w[i + 1]);
+    if (NW == 2) {
+      pf[NW - 1][r >> 3][(r & 7) + i] = (_Float16)__builtin_fmaf((float)h[0], minus, w[i]);
+      pf[NW - 1][r >> 3][(r & 7) + i + 1] = (_Float16)__builtin_fmaf((float)h[1], minus, w[i + 1]);
     }
   }
   return (w[0] + w[1]) + (w[2] + w[3]);
 }
 // ... of all 16, and their sum into l.
-template <int NP>
+template <int NW>
 T2R_DEV void soft_exp(const v16f_t& s, float sk, float add, const Bases& b, float& l, v8h_t (*pf)[2]) {
   float ls = 0;
 #pragma unroll
-  for (int r = 0; r < 16; r += 4) ls += soft_weights<NP>(s, sk, add, pf, r);
+  for (int r = 0; r < 16; r += 4) ls += soft_weights<NW>(s, sk, add, pf, r);
   l = add_weights(l, ls, add, b);
 }
 
@@ -673,7 +680,7 @@ T2R_DEV int plain_steps(long long all_see, long long seg, int n, int step, bool 
 
 template <class E, int HD>
 __global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_few(BlkAttn p) {
-  constexpr int NP = Pieces<E>::kN, KU = HD / 32, DT = HD / 32;
+  constexpr int NQ = Pieces<E>::kQ, NW = Pieces<E>::kW, KU = HD / 32, DT = HD / 32;
   __shared__ BaSeg sg;
   using End = TileEnd<HD, 1, 1>;
   __shared__ typename End::Ml ml;
@@ -688,7 +695,7 @@ __global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_few(BlkAtt
   int blk = seg_table(p.c, t.s.b, k0, (int)min((long long)kBaSeg, kend - k0));
   float x[KU][16];
   q_load<E, KU>((const E*)p.q + col_at(t, G, hd, kvh, cc, p.q_ld), hd, x);
-  v8h_t qf[KU][NP][2];
+  v8h_t qf[KU][NQ][2];
   const long long at = t.s.p0 + t.i0 + cc / G, all_see = t.s.p0 + t.i0 + 1;   // (keys below all_see are seen by every row)
   // row 8 i + 4 c' + r of the 32 stands for key 16 c' + 4 i + r
   const int kc = (col >> 2) & 1, krow = 4 * (col >> 3) + (col & 3);
@@ -733,23 +740,23 @@ __global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_few(BlkAtt
         for (int half = 0; half < 2; ++half) {
           const v8h_t kf = codes_h(kr[u][2 * half], kr[u][2 * half + 1]);
 #pragma unroll
-          for (int q = 0; q < NP; ++q) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[u][q][half], s, 0, 0, 0);
+          for (int q = 0; q < NQ; ++q) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[u][q][half], s, 0, 0, 0);
         }
       const bool more = st + kBaWaves < steps;
       if (more) load_k(st + kBaWaves);
       const int ch = st * 2 + c2;
-      v8h_t pf[NP][2];
+      v8h_t pf[NW][2];
       const float sk = score_scale(sq, sg.ks[ch]);
       const float add = soft_max<DT, edge.value>(s, sk, edge.value ? keys_left(at, seg + ch * 16, sg.seen[ch]) : 16, sg.ue[ch],
                                                  sg.uf[ch], bs, l, o[0]);
-      soft_exp<NP>(s, sk, add, bs, l, pf);
+      soft_exp<NW>(s, sk, add, bs, l, pf);
 #pragma unroll
       for (int i = 0; i < DT; ++i)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const v8h_t vf = codes_h(vr[i][2 * half], vr[i][2 * half + 1]);
 #pragma unroll
-          for (int q = 0; q < NP; ++q) o[0][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[q][half], o[0][i], 0, 0, 0);
+          for (int q = 0; q < NW; ++q) o[0][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[q][half], o[0][i], 0, 0, 0);
         }
       if (more) load_v(st + kBaWaves);
     };
@@ -774,7 +781,7 @@ __global__ __launch_bounds__(kBaThreads, HD == 64 ? 3 : 2) void k_blk_few(BlkAtt
 // before the softmax, and two buffers leave one barrier a stage.
 template <class E, int HD, int CT>
 __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
-  constexpr int NP = Pieces<E>::kN, KU = HD / 32, DT = HD / 32, CG = 2, KG = kBaWaves / CG, COLS = 32 * CT * CG;
+  constexpr int NQ = Pieces<E>::kQ, NW = Pieces<E>::kW, KU = HD / 32, DT = HD / 32, CG = 2, KG = kBaWaves / CG, COLS = 32 * CT * CG;
   constexpr int STAGE = 32 * KG, FR = KG * KU * 2, PIECES = STAGE * HD / 16, PER = PIECES / kBaThreads;   // 16-byte pieces of K, of V
   using End = TileEnd<HD, CT, CG>;
   constexpr int kBufs = 4 * FR * 1024;
@@ -791,7 +798,7 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
   if (!tile_of<E>(p, COLS, &t, &kvh, &k0, &kend)) return;
   const int ncol = t.rows * G;
   int blk = seg_table(p.c, t.s.b, k0, (int)min((long long)kBaSeg, kend - k0));
-  v8h_t qf[CT][KU][NP][2];
+  v8h_t qf[CT][KU][NQ][2];
   float x[CT][KU][16], sq[CT], l[CT];
   Bases bs[CT];
   long long at[CT];
@@ -883,7 +890,7 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g) {
 #pragma unroll
-        for (int q = 0; q < NP; ++q)
+        for (int q = 0; q < NQ; ++q)
 #pragma unroll
           for (int ct = 0; ct < CT; ++ct) s[ct] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[g >> 1][g & 1], qf[ct][g >> 1][q][g & 1], s[ct], 0, 0, 0);
         if (g == 0) read_k(KU / 2, KU);
@@ -897,7 +904,7 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
       };
       read_v(0);
       __builtin_amdgcn_sched_barrier(0);
-      v8h_t pf[CT][NP][2];
+      v8h_t pf[CT][NW][2];
       float sk[CT], add[CT], ls[CT];
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
@@ -909,7 +916,7 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
       // The probabilities of 8 keys, then their products; the other 8 keys' between those, the next loads between the last.
       auto weigh = [&](int r) {
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) ls[ct] += soft_weights<NP>(s[ct], sk[ct], add[ct], pf[ct], r);
+        for (int ct = 0; ct < CT; ++ct) ls[ct] += soft_weights<NW>(s[ct], sk[ct], add[ct], pf[ct], r);
       };
 #pragma unroll
       for (int r = 0; r < 8; r += 4) weigh(r);
@@ -917,14 +924,14 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
 #pragma unroll
       for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int g = 0; g < NP * DT; ++g) {
+        for (int g = 0; g < NW * DT; ++g) {
           const int q = g / DT, i = g % DT;
 #pragma unroll
           for (int ct = 0; ct < CT; ++ct) o[ct][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[i][half], pf[ct][q][half], o[ct][i], 0, 0, 0);
           if (half == 0) {
             if (g == 0) read_v(1);
 #pragma unroll
-            for (int r = 2 + g * 2 / (NP * DT); r < 2 + (g + 1) * 2 / (NP * DT); ++r) weigh(4 * r);
+            for (int r = 2 + g * 2 / (NW * DT); r < 2 + (g + 1) * 2 / (NW * DT); ++r) weigh(4 * r);
           } else if (g == 0) {
             load_k(min(st + 2, last));
           } else if (g == 1) {

@@ -227,7 +227,7 @@ int t2r_attn_blk_decode(const void* q, int dtype, int64_t q_ld, const int8_t* kc
   const hipStream_t st = (hipStream_t)stream;
   return by_type(dtype, [&](auto e) {
     using E = decltype(e);
-    const int sets = (p.G + Pieces<E>::kHeads - 1) / Pieces<E>::kHeads;
+    const int heads = 16 / Pieces<E>::kQ, sets = (p.G + heads - 1) / heads;
     // later parts come last: those past their sequence's end, which return at once, then hold up nobody's place
     const dim3 grid(Hk * sets, B, cut.nsplit);
     if (hd <= 64) launch((k_blk_step<E, 64>), grid, dim3(kBaThreads), 0, st, p);
