@@ -426,12 +426,12 @@ T2R_DEV float join_parts(const BlkAttn& p, long long at, int parts, float (*x)[2
   }
   return l;
 }
-// two channels of a joined row; place: it stands in its sequence
+// Two channels of a joined row. (It has a place in its sequence: a tile in parts ends past 512 keys and has 128 rows at most.)
 template <class E>
-T2R_DEV void join_store(const BlkAttn& p, E* out, const float* x, float l, const Bases& top, bool place) {
+T2R_DEV void join_store(const BlkAttn& p, E* out, const float* x, float l, const Bases& top) {
   const int d = 2 * (threadIdx.x & 63);
   if (d >= p.c.hd) return;
-  const float inv = !place ? fv(kQNaN) : l == 0 ? 0.0f : 1.0f / l;
+  const float inv = l == 0 ? 0.0f : 1.0f / l;
   const int e = base_shift(top);
   out[d] = narrow<E>(__builtin_amdgcn_ldexpf(x[0] * inv, e));
   out[d + 1] = narrow<E>(__builtin_amdgcn_ldexpf(x[1] * inv, e));
@@ -447,7 +447,7 @@ __global__ __launch_bounds__(kBaThreads) void k_blk_step_join(BlkAttn p) {
   float x[2];
   Bases top;
   const float l = join_parts<kBaWaves>(p, ((long long)b * p.H + h) * p.nsplit, parts, &x, &top);
-  if (wave_index() == 0) join_store<E>(p, (E*)p.out + (long long)b * p.out_ld + (long long)h * p.c.hd, x, l, top, true);
+  if (wave_index() == 0) join_store<E>(p, (E*)p.out + (long long)b * p.out_ld + (long long)h * p.c.hd, x, l, top);
 }
 
 // ---------------------------------------------------------------- several rows a sequence
@@ -882,7 +882,7 @@ __global__ __launch_bounds__(kBaThreads, 2) void k_blk_tile(BlkAttn p) {
       __builtin_amdgcn_sched_barrier(0);
       // The scores; between their products the next stage's codes are converted. (The order is pinned: left to itself the
       // compiler puts all of one before all of the other.)
-            v16f_t s[CT];
+      v16f_t s[CT];
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) s[ct] = v16f_t{};
       constexpr int GROUPS = KU * 2, EACH = 4 * PER / GROUPS;
@@ -970,7 +970,7 @@ __global__ __launch_bounds__(kBaThreads) void k_blk_rows_join(BlkAttn p, int col
   Bases top;
   const float l = join_parts<NWV>(p, ((long long)blockIdx.x * cols + cc) * p.nsplit, parts, &x, &top);
   if (NWV == 1 || wave_index() == 0)
-    join_store<E>(p, (E*)p.out + col_at(t, p.G, p.c.hd, kvh, cc, p.out_ld), x, l, top, t.s.p0 + t.i0 + cc / p.G >= 0);
+    join_store<E>(p, (E*)p.out + col_at(t, p.G, p.c.hd, kvh, cc, p.out_ld), x, l, top);
 }
 
 }  // namespace t2r
