@@ -70,6 +70,13 @@ def test_attention_refuses_its_own():
     assert lib.t2r_attn_blk_workspace_bytes(1, 0, 5, 2, 64, 64, 128, 0) == -1
 
 
+@pytest.mark.parametrize("form", ["decode", "prefill"])
+def test_attention_refuses_scales_past_the_kernels_range(form):
+    """The kernels take scale log2(e): an infinity there would give NaN where q or a key is zero."""
+    for scale, code in ((2.9e38, abi.T2R_EINVAL), (2.3e38, abi.T2R_ENOMEM)):       # (a second refusal follows: no workspace)
+        assert attend(abi.load(), form, scale=scale, width=64) == code
+
+
 @pytest.mark.parametrize("sizes", [
     (384, 384, 1, 1, 64, 1 << 30, 1 << 30, 0),                             # (a cut of 2^32 keys is 0 in 32 bits)
     (1, 0, 4, 2, 64, 48, 100, 0), (1, 0, 4, 2, 72, 64, 100, 0), (1, 0, 4, 2, 144, 64, 100, 0), (1, 0, 4, 2, 64, 128, 1 << 24, 0),

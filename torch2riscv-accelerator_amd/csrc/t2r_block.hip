@@ -118,6 +118,8 @@ Cut rows_cut(int B, int rows, int H, int Hk, int hd, int block, int width) {
   return c;
 }
 
+// (the kernels take it times log2(e))
+bool scale_ok(float scale) { return scale > 0 && scale * kLog2e <= 3.4028234663852886e38f; }
 bool attn_shape_ok(int H, int Hk) { return Hk > 0 && H > 0 && H % Hk == 0 && H / Hk <= 32; }
 // The two forms' sizes, of the calls and of the workspace query alike (the cuts are worked out for these only); the cut, or
 // false where a launch cannot hold it
@@ -209,7 +211,7 @@ int t2r_attn_blk_decode(const void* q, int dtype, int64_t q_ld, const int8_t* kc
                         const float* vs, int n_blocks, int block, int Hk, int hd, const int32_t* table, int width,
                         const int32_t* lens, int B, int H, float scale, void* out, int64_t out_ld, void* workspace,
                         int64_t workspace_bytes, void* stream) {
-  if (!q || !out || !lens || !dtype_ok(dtype) || !(scale > 0) || scale > 3.0e38f) return T2R_EINVAL;
+  if (!q || !out || !lens || !dtype_ok(dtype) || !scale_ok(scale)) return T2R_EINVAL;
   if (misaligned(q, elem_size(dtype)) || misaligned(out, elem_size(dtype)) || misaligned(lens, 4)) return T2R_EINVAL;
   BlkAttn p;
   std::memset(&p, 0, sizeof(p));
@@ -220,7 +222,7 @@ int t2r_attn_blk_decode(const void* q, int dtype, int64_t q_ld, const int8_t* kc
   if (need > 0 && (!workspace || workspace_bytes < need || misaligned(workspace, 16))) return T2R_ENOMEM;
   p.q = q; p.q_ld = q_ld; p.out = out; p.out_ld = out_ld;
   p.g = Ragged{nullptr, lens, B, B};
-  p.H = H; p.G = H / Hk; p.a = scale * 1.44269504f;
+  p.H = H; p.G = H / Hk; p.a = scale * kLog2e;
   p.chunk = cut.chunk; p.nsplit = cut.nsplit;
   p.ws_o = (float*)workspace;
   p.ws_ml = p.ws_o + (long long)B * H * cut.nsplit * hd;
@@ -241,7 +243,7 @@ int t2r_attn_blk_prefill(const void* q, int dtype, int64_t q_ld, const int8_t* k
                          const float* vs, int n_blocks, int block, int Hk, int hd, const int32_t* table, int width,
                          const int32_t* starts, const int32_t* lens, int B, int rows, int H, float scale, void* out,
                          int64_t out_ld, void* workspace, int64_t workspace_bytes, void* stream) {
-  if (!q || !out || !starts || !lens || !dtype_ok(dtype) || !(scale > 0) || scale > 3.0e38f) return T2R_EINVAL;
+  if (!q || !out || !starts || !lens || !dtype_ok(dtype) || !scale_ok(scale)) return T2R_EINVAL;
   if (misaligned(q, elem_size(dtype)) || misaligned(out, elem_size(dtype)) || misaligned(starts, 4) || misaligned(lens, 4)) return T2R_EINVAL;
   BlkAttn p;
   std::memset(&p, 0, sizeof(p));
@@ -252,7 +254,7 @@ int t2r_attn_blk_prefill(const void* q, int dtype, int64_t q_ld, const int8_t* k
   if (need > 0 && (!workspace || workspace_bytes < need || misaligned(workspace, 16))) return T2R_ENOMEM;
   p.q = q; p.q_ld = q_ld; p.out = out; p.out_ld = out_ld;
   p.g = Ragged{starts, lens, B, rows};
-  p.H = H; p.G = H / Hk; p.a = scale * 1.44269504f;
+  p.H = H; p.G = H / Hk; p.a = scale * kLog2e;
   p.chunk = cut.chunk; p.nsplit = cut.nsplit;
   p.order = (long long)cut.tiles * Hk <= 512 ? ORDER_BOTH : ORDER_BACKWARDS;
   p.ws_o = (float*)workspace;
