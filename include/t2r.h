@@ -170,9 +170,9 @@ enum { T2R_F32 = 0, T2R_BF16 = 1, T2R_F16 = 2 };
  *   kc [n_blocks, Hk, block, hd], ks [n_blocks, Hk]: key   = F(code * scale)
  *   vc [n_blocks, Hk, hd, block], vs [n_blocks, Hk]: value = F(code * scale)   (by channel: the attention reads along tokens)
  *   table [B, width]: position p of sequence b lies in block table[b, p / block], slot p % block.
- * hd <= 128 and a multiple of 16; kc and vc start on 16 bytes. A table entry outside [0, n_blocks), and a place past the
- * table, holds no tokens: appended rows are dropped there, the attention leaves its positions out, reads give zeros.
- * A block that is appended to stands in one place of one sequence (full blocks may be shared by tables).
+ * Scales are not negative. hd <= 128 and a multiple of 16; kc and vc start on 16 bytes. A table entry outside [0, n_blocks),
+ * and a place past the table, holds no tokens: appended rows are dropped there, the attention leaves its positions out, reads
+ * give zeros. A block that is appended to stands in one place of one sequence (full blocks may be shared by tables).
  * Ragged rows: those of sequence b are starts[b] .. starts[b + 1] - 1 (starts [B + 1], device, not decreasing) and the
  * last of them stands at position lens[b] - 1 (device); rows outside every sequence are left alone. rows < 2^24.
  *

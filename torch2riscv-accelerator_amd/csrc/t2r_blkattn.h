@@ -175,8 +175,10 @@ T2R_DEV int base_shift(const Bases& b) { return (int)(b.M - b.m); }
 //
 // Every code is needed once, so the codes go from memory into the waves' registers, a step ahead, and never through LDS; the
 // loads of a step are 64 tokens' whole rows. Long caches are bound by memory: 32 sequences of 8192 tokens, 8 KV heads of 128,
-// 5.4 TB/s; of 1021 .. 8192 tokens 63 us (4.8 TB/s: the longest sequences end alone) and 4.3 for the join. Short ones are a
-// chain of length, table, scales, codes and products: one sequence of 96 tokens 4.5 us, of 8101 5.9 and 4.4.
+// 98 us (5.5 TB/s); of 1021 .. 8192 tokens 60 (5.0 TB/s: the longest sequences end alone), 58 for bf16 rows, and 4.4 for the join.
+// Short ones are a chain of length, table, scales, codes and products: one sequence of 96 tokens 4.7 us, of 8101 5.9 and 4.7.
+// Head dims between 64 and 128, and below 64, run as the next of these: their codes alone are read, but a wave's chain is as
+// long, so the same lengths of 4 heads of 80 take 28 us (3.4 TB/s), of 5 of 96 30 (4.7), of 7 of 32 27 (2.4).
 //
 // fp16 pieces of an fp32 number: of q, of the weights of the ragged form. One piece of a weight is 2^-12 off, which fp16 results
 // show (2-norm, 2.9e-4 off against 2.06e-4 of the rounded exact ones and of two pieces) and bf16's do not (1.67e-3, 1.65e-3,
@@ -456,18 +458,20 @@ __global__ __launch_bounds__(kBaThreads) void k_blk_step_join(BlkAttn p) {
 //
 // k_blk_few: 32 columns. The four waves take every fourth 32 keys, each loading and converting its codes by itself: nothing
 // is shared but the columns, and no barrier stands in the loop. 8 rows of each of four sequences over 5003 .. 8100 positions,
-// 32 heads of 64: 16 us in parts of 512 keys, of which a part's beginning and end are half, and 5.4 for the join.
+// 32 heads of 64: 16 us in parts of 512 keys, of which a part's beginning and end are half, and 5.1 for the join.
 // k_blk_tile: 64 CT columns, two groups of 32 CT for the waves; the two waves of a group take the stage's two times 32 keys. The
 // workgroup loads a stage's codes together (a stage ahead), converts them once into LDS, in the MFMA operands' order, two
 // stages in turn with one barrier each. The conversion is as much vector work as the softmax of 32 columns (80 instructions of
 // 32 keys at head dim 128 where two waves share it, against 100), so the groups share it.
 // Bound by issue: a product takes 32 cycles of its unit and a vector instruction 4, five where a SIMD has one wave, and beyond
-// three a product they add up. At head dim 128 in fp32 a wave has 32 products and 194 other vector instructions a stage, in
-// bf16 at 64 16 and 180. One prompt of 2032 rows, 16 heads of 128 in fp32: 53 us (318 TFLOP/s of the formula's, twice that of
-// fp16 products, q and p being two pieces), 1.17 us a stage where one workgroup is on a CU, 1.03 where two are, so each CU's
-// 33 stages take about as long however tiles are cut or paired; 7 us a tile lie before and after them. Seven prompts and turns
-// in bf16, 32 heads of 64: 74 us (488 TFLOP/s). Slower, all measured: eight waves a workgroup, a second stage in flight in
-// registers, tiles cut along their keys; four groups of 32 columns at head dim 128 gain 0 .. 10% past 8000 rows and lose before.
+// three a product they add up. At head dim 128 in fp32 a wave has 32 products and 200 other vector instructions a stage, in
+// bf16 at 64 16 and 215. One prompt of 2032 rows, 16 heads of 128 in fp32: 49.8 us in a row of calls (340 TFLOP/s of the formula's,
+// twice that of fp16 products, q and the weights being two pieces), some 1.2 us a stage where one workgroup is on a CU, 1.0 where
+// two are, so each CU's 33 stages take about as long however tiles are cut or paired; 7 us a tile lie before and after them. Seven
+// prompts and turns in bf16, 32 heads of 64, 37.2 GFLOP: 68.7 us (541 TFLOP/s). Slower, all measured: eight waves a workgroup, a
+// second stage in flight in registers, tiles cut along their keys; four groups of 32 columns at head dim 128 gain 0 .. 10% past
+// 8000 rows and lose before. Other head dims run as 64 or 128 with the products of the missing channels: the prompt of 2032 rows
+// of 16 heads takes 45.5 us at head dim 80 and 48.8 at 96, 31.0 and 30.9 at 48 and 32 against 32.0 at 64.
 struct Tile {
   Seq s;
   int t, i0, rows;          // tile t of sequence s: its rows i0 .. i0 + rows - 1

@@ -206,7 +206,8 @@ T2R_DEV int quant_code(float x, float s, float inv) {
   q = fminf(fmaxf(q, -127.0f), 127.0f);
   return x != x ? 0 : (int)q;
 }
-// The same where it is plain. y after its step is the quotient rounded, and exact where that is a fp32 number, as ties are: so
+// The same where it is plain. y after its step (a quotient by a reciprocal and one fused remainder: Markstein's division) is the
+// quotient rounded, and exact where that is a fp32 number, as ties are: so
 // rintf settles them, and a remainder of at most half a step says that no other integer is nearer. *sure is cleared where it
 // is not that (NaN, an infinity, and without FIX a quotient rounded past the middle): quant_code then. FIX is for 16-bit rows,
 // where that is no rarity: half of the largest value is often among them, 63.5 steps but for the scale's rounding. (All by
@@ -251,7 +252,7 @@ T2R_DEV uint32_t byte_mask(int i, int from, int to) {
 // one launch do. A thread has NU units of 16 values, which stay in registers between the maximum and the codes: K (token,
 // 16 channels), V (channel, 16 tokens: lanes along the channels, so that loads are whole lines and a store is 16 codes).
 // Reads the rows, writes a byte a value. A call of few rows is a launch and one chain of loads (16 sequences of 8 heads of 64,
-// a row each: 4.2 us, 3.3 of them an empty kernel's); a prompt of 2032 rows of 8 heads of 128 in fp32 takes 9.2 us (2.3 TB/s
+// a row each: 4.5 us, 3.3 of them an empty kernel's); a prompt of 2032 rows of 8 heads of 128 in fp32 takes 8.3 us (2.5 TB/s
 // of 20.8 MB, 508 workgroups: loads, maximum, codes and stores follow each other in each, and all run at once).
 template <class E, int NU>
 __global__ __launch_bounds__(kBlkThreads) void k_blk_append(BlkRows x, Ragged g, BlkCache c) {
@@ -348,7 +349,8 @@ __global__ __launch_bounds__(kBlkThreads) void k_blk_append(BlkRows x, Ragged g,
 }
 
 // Rows out of the cache, as the values that the codes stand for; zeros where the table holds no such position. The same
-// pieces as above, the other way. 2032 rows of 8 heads of 128 to fp32: 8.9 us (2.3 TB/s); single rows 4.6 us.
+// pieces as above, the other way. 2032 rows of 8 heads of 128 to fp32: 8.2 us in a row of calls, 9.7 from idle (20.8 MB, 2.1 to
+// 2.5 TB/s: table, scale, codes and stores of 508 workgroups, once each); single rows 4.5 us.
 template <class E>
 __global__ __launch_bounds__(kBlkThreads) void k_blk_read(Ragged g, BlkCache c, E* k, E* v) {
   const int tid = threadIdx.x, head = blockIdx.y, hd = c.hd, lbs = c.lbs;

@@ -87,8 +87,11 @@ Cut rows_cut(int B, int rows, int H, int Hk, int hd, int block, int width) {
   Cut c;
   // Few rows: one tile of 32 columns a sequence. Else 64; 128, which a conversion of codes then serves, at head dims whose sums
   // leave a wave registers for two times 32, once 64 would be more than the chip has places for twice (1024). 32 heads of 64,
-  // one prompt of 512 / 2032 / 4064 rows, us: fp32 13.1 / 51.4 / 175 in 64 columns and 18.0 / 52.5 / 156 in 128, bf16 11.2 /
-  // 40.1 / 122 and 15.1 / 40.0 / 111.
+  // one prompt of 512 / 2032 / 4064 rows, us: fp32 13.2 / 51.1 / 162 in 64 columns and 22.6 / 51.8 / 153 in 128, bf16 12.3 /
+  // 38.0 / 116 and 19.6 / 37.7 / 105, fp16 12.3 / 43.2 / 141 and 20.8 / 44.2 / 131. One rule for the whole call: a batch of a prompt
+  // and single rows has the prompt's columns for all of them, a prompt among many idle sequences 32. 31 rows at 1000 .. 8192
+  // positions and a prompt of 512 in bf16 take 95 us in one call, 32 and 16 in two (the rows by the step form); 2000 rows among
+  // 256 slots 50, alone 38.
   c.cols = (long long)rows * G <= 32LL * B ? 32 : hd <= 64 && (long long)rows * H > 64 * 1024 ? 128 : 64;
   const int rt = c.cols / G;
   // every sequence's last tile may be a part of one
@@ -98,14 +101,15 @@ Cut rows_cut(int B, int rows, int H, int Hk, int hd, int block, int width) {
   c.nsplit = 1;
   // A part costs what a tile costs before and after its keys (7 us) and the join's launch (4 to 5 us); 64 keys of a tile take 1.3
   // us. So keys are cut only while workgroups leave half of the chip's places empty, and into parts of 512 at least: a
-  // 1024-row prompt (256 workgroups) took 30 + 13 us in four parts and 31 whole, 8 rows at 8100 positions 200 us whole.
+  // 1024-row prompt (256 workgroups) took 33 us in four parts and 26 whole, 8 rows at 8100 positions 16 in parts and 52 whole.
   // Few rows are one tile a sequence as a rule, three workgroups of which fit a CU: 8 rows of 16 sequences at 5000 .. 8100
-  // positions, 32 heads of 64, took 46 / 36 / 33 / 37 / 46 us in parts of 4096 / 2048 / 1280 / 1024 / 512 keys; of 4
-  // sequences 23 / 21 / 21 in parts of 2048 / 1024 / 512.
+  // positions, 32 heads of 64, took 52 / 41 / 35 / 38 / 48 us in parts of 4096 / 2048 / 1280 / 1024 / 512 keys; of 4
+  // sequences 23 / 21 / 20 in parts of 2048 / 1024 / 512.
   // Turns of a few hundred rows late in long caches (tables past 2048 positions) gain from a second workgroup on every CU, in
-  // parts of 1536 at least: 548 rows at 7127 positions, 32 heads of 64 in bf16 (280 workgroups), took 103 us whole and 86 / 81 /
-  // 80 / 78 / 83 in parts of 4096 / 2688 / 2048 / 1536 / 1024; 1200 at 8000, 16 heads of 128 (304), 160 and 148 / 141 / 138 / 141 /
-  // 152; but 900 rows (456) 99 whole and 111 to 123 in parts.
+  // parts of 1536 at least: 548 rows at 7127 positions, 32 heads of 64 in bf16 (280 workgroups), took 97 us whole and 79 / 77 /
+  // 73 / 72 / 77 in parts of 4096 / 2688 / 2048 / 1536 / 1024; 1200 at 8000, 16 heads of 128 (304) in bf16, 151 and 143 / 128 / 128 /
+  // 130 / 138; but 900 rows (456) 95 whole and 107 to 109 in parts. The lengths are on the device, so a first prompt of some hundred
+  // rows in such a table pays for parts that it has not got: 512 rows 16.3 us, 12.4 whole (fp32 17.5 and 12.7).
   const bool few = c.cols == 32;
   const long long wgs = (few ? B : tiles) * Hk;
   const bool turns = !few && wgs > 128 && cap > 2048;

@@ -6,8 +6,8 @@
 //
 // fp32 logits are bound by memory (1024 rows of 151936, top 20: 116 us, 5.4 TB/s), 16-bit ones by the vector units: six
 // instructions a value, one of them an exponential that counts four times, and what a span needs besides. 2032 rows of 49155:
-// 51 us with the top 5 (3.9 TB/s), 42 without; of 128256: 110 us with the top 20 (4.7), 101 without. Few rows: 16 of 128256
-// 7.0 us and 6.6 for the join, an empty kernel taking 3.3.
+// 48 us with the top 5 (4.2 TB/s), 42 without; of 128256: 110 us with the top 20 (4.7), 101 without. Few rows: 16 of 128256
+// 7.7 us and 6.3 for the join, an empty kernel taking 3.3. Small vocabularies with a large top are slow (the selection below).
 #pragma once
 #include "t2r_block.h"
 
@@ -179,7 +179,9 @@ __global__ __launch_bounds__(kLpThreads, 4) void k_lp_part(LpArgs p) {
     __syncthreads();
     int nk = s.keys;
     if (nk > kLpKeys) {
-      // too many (equal values, say): the largest one by one
+      // Too many: the largest one by one. Equal values, or rows whose values lie with fewer threads than the first span's bound
+      // has groups for, so that every value is a candidate: 513 to 608 values of 16 bits with the top 20, 513 to 992 with the top
+      // 32. (2032 such rows of 600: 140 and 210 us; of 500, by rank among 500 keys, 87; of 1000 with the top 20, under a bound, 15.)
       unsigned long long below = ~0ull;
       for (nk = 0; nk < top; ++nk) {
         unsigned long long b = 0;
@@ -350,7 +352,7 @@ __global__ __launch_bounds__(kLpThreads) void k_lp_join(LpArgs p) {
   v4f_t sum = {kLpNone, 0, 0, 0};
   unsigned long long last = 0;
   const unsigned long long* from = p.ws_key + (long long)row * parts * top;
-  // (the token's logit and the keys are asked for before anything waits)
+  // (the token is waited for, for its range; then its logit, the keys and the sums are asked for together)
   float xt = fv(kQNaN);
   if (p.logprob) xt = lp_logit<E>(p, row);
   constexpr int KEYS = kLpMaxParts * kLpMaxTop / kLpThreads;

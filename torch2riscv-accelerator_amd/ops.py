@@ -291,7 +291,8 @@ def kv_append_block(k, v, kc, vc, ks, vs, table, starts, lens):
     """Rows k, v [rows, Hk * hd] into the cache (t2r_kv_append_blk): those of sequence b are starts[b] .. starts[b + 1] - 1
     and the last of them gets position lens[b] - 1 (lens counts them). A block's scale for a head is max |x| / 127 over what
     it holds; it grows with later rows, and the block's earlier codes then move to it. Rows at places that the table has
-    no block for are dropped."""
+    no block for are dropped. A block that rows enter stands in one place of one sequence: what two sequences share are full
+    blocks, and a copy of the last one is the caller's."""
     n = kc.shape[1] * kc.shape[3] if kc.dim() == 4 else 0
     k_ld, code, dev = _rows(k, n, "k")
     v_ld, vcode, vdev = _rows(v, n, "v")
